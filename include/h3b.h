@@ -46,7 +46,7 @@ extern "C" {
 #define H3B_STATUS_OK 0
 #define H3B_STATUS_MBAR_TIMEOUT 1 /* a GEMM pipeline wait ran out (kernel aborted its tile loop) */
 #define H3B_STATUS_PEER_TIMEOUT 2 /* a peer barrier wait ran out (a rank did not arrive) */
-#define H3B_STATUS_BAD_INDEX 3    /* a modulation row index was outside [0, R) (row skipped) */
+#define H3B_STATUS_BAD_INDEX 3    /* a modulation row or key block index was out of range (row or block skipped) */
 
 H3B_API int h3b_abi_version(void);
 H3B_API const char *h3b_last_error(void);
@@ -243,6 +243,68 @@ H3B_API int h3b_gate_norm_mod_quant_(void *x, const void *o, const void *g, cons
  * Replaces gate_, h3_fuse_kernels.py:188-192 (kernel :158-167). */
 H3B_API int h3b_gate_(void *x, const void *o, const void *g, const int32_t *ridx, int64_t S, int64_t D, int64_t R,
               void *stream);
+
+/* ---- attention ----------------------------------------------------------- */
+/* These take the place of the scaled_dot_product_attention call between the
+ * qkv and the out projection (sp_forward.py:276-318).  q, k, v, o bf16
+ * [tokens, H, D], D 64 or 128: `_ld` is the stride between tokens and `_hs`
+ * the stride between heads, in elements, positive multiples of 8; every start
+ * is 16-byte aligned.  Sizes are host values: a captured launch keeps them. */
+
+/* Quantise n tokens of k and v into tokens start .. start + n of a cache:
+ * codes kq, vq int8 [H, cap, D], scales ks, vs fp32 [H, cap / 64], cap % 64 == 0.
+ * Per block of 64 tokens and head, K and V apart: s = max|x| / 127 over the new
+ * tokens (IEEE division), or the block's former scale if tokens before `start`
+ * stay in the block and it is larger; code = clamp(rint_half_even(x / s),
+ * -127, 127), 0 for s = 0; staying codes become rint(code * (former / s)) if the
+ * scale grew.  A NaN or infinity makes its block's scale non-finite and the
+ * codes 0.  Nothing behind start + n is written.  The cross-attention's K / V
+ * projection is the same in every denoising step; the reference recomputes
+ * it (the attention call of sp_forward.py:276-318). */
+H3B_API int h3b_kv8_write(const void *k, int64_t k_ld, int64_t k_hs, const void *v, int64_t v_ld, int64_t v_hs,
+                          int64_t start, int64_t n, int64_t H, int64_t D, int8_t *kq, int8_t *vq, float *ks,
+                          float *vs, int64_t cap, void *stream);
+
+/* The values code * scale of tokens start .. start + n of such a cache ->
+ * k_out, v_out [n, H, D] contiguous, fp32 if `fp32` is set, otherwise rounded
+ * to bf16: what the attention of sp_forward.py:276-318 would be given. */
+H3B_API int h3b_kv8_read(const int8_t *kq, const int8_t *vq, const float *ks, const float *vs, int64_t cap,
+                         int64_t start, int64_t n, int64_t H, int64_t D, void *k_out, void *v_out, int fp32,
+                         void *stream);
+
+/* o = softmax(scale * q K^T) V over the first `length` tokens of such a cache
+ * (K = kq * ks, V = vq * vs); length 0 gives zeros.  Replaces the
+ * scaled_dot_product_attention of sp_forward.py:276-318 where K and V are kept. */
+H3B_API int h3b_kv8_attn(const void *q, int64_t q_ld, int64_t q_hs, int64_t Sq, int64_t H, int64_t D,
+                         const int8_t *kq, const int8_t *vq, const float *ks, const float *vs, int64_t cap,
+                         int64_t length, float scale, void *o, int64_t o_ld, int64_t o_hs, void *stream);
+
+/* out[b, h, :] = mean of rows b * rows .. of x [S, H, D] bf16 (rows 64 or 128;
+ * the last block over the rows it has) -> fp32 [ceil(S / rows), H, D], summed
+ * in 64 bits and rounded once.  The cheap score of block-sparse attention in
+ * place of the dense one of sp_forward.py:276-318. */
+H3B_API int h3b_block_means(const void *x, int64_t ld, int64_t hs, int64_t S, int64_t H, int64_t D, int64_t rows,
+                            float *out, void *stream);
+
+/* blocks[h, i, 0 .. topk) = the j with the largest qm[i, h, :] . km[j, h, :]
+ * (64-bit sums; ties to the lowest j, NaN below every number), ascending.
+ * qm fp32 [nq, H, D], km fp32 [nk, H, D], 0 <= topk <= nk.  The scores pass
+ * through `workspace`, in as many rounds as it takes to fit
+ * (h3b_select_blocks_workspace gives a size; 512 * nk bytes is the least).
+ * Chooses what the attention of sp_forward.py:276-318 is restricted to. */
+H3B_API int64_t h3b_select_blocks_workspace(int64_t nq, int64_t nk, int64_t H);
+H3B_API int h3b_select_blocks(const float *qm, const float *km, int64_t nq, int64_t nk, int64_t H, int64_t D,
+                              int64_t topk, int32_t *blocks, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* o = softmax(scale * q K^T) V, query rows 128 i .. 128 i + 127 of head h over
+ * the keys of blocks[h, i, 0 .. topk) only; block b holds keys 64 b .. 64 b + 63
+ * below Sk.  -1 is no block; another index out of range is skipped and recorded
+ * as H3B_STATUS_BAD_INDEX; a block named twice counts twice; rows without a key
+ * are zero.  Replaces the scaled_dot_product_attention of sp_forward.py:276-318. */
+H3B_API int h3b_block_sparse_attn(const void *q, int64_t q_ld, int64_t q_hs, int64_t Sq, int64_t H, int64_t D,
+                                  const void *k, int64_t k_ld, int64_t k_hs, const void *v, int64_t v_ld,
+                                  int64_t v_hs, int64_t Sk, const int32_t *blocks, int64_t topk, float scale,
+                                  void *o, int64_t o_ld, int64_t o_hs, void *stream);
 
 /* ---- Ulysses all-to-all -------------------------------------------------- */
 

@@ -1,0 +1,225 @@
+// Key/value cache held in 8 bits: quantise while writing, and read back.
+//
+// codes [H, cap, D] int8, scales [H, cap / 64] fp32, K and V apart: the tokens
+// of one head lie together, so a tile of any 128 tokens that the attention
+// takes is one contiguous run, and a block of 64 tokens of a head (what shares
+// a scale) is 64 * D consecutive bytes.
+//
+//   scale = max |x| / 127 over the block's new tokens (IEEE division), or the
+//           block's older scale where older tokens stay and it is larger;
+//   code  = clamp(rint_half_even(x / scale), -127, 127), 0 for scale 0;
+//   codes that stay are requantised, rint(code * (old / scale)), if the scale grew.
+// A non-finite x makes the scale non-finite and the block's codes 0, so
+// everything read from it is NaN.  Maxima run on the bit patterns of |x|,
+// which order NaN above infinity above the numbers.
+#include "common.cuh"
+
+namespace h3b {
+namespace kv8 {
+
+constexpr int kBlock = 64;  // tokens per scale
+constexpr int kThreads = 256;
+
+struct WriteArgs {
+    const uint16_t* x[2];  // k, v: [n, H, D], strides in elements
+    int64_t ld[2], hs[2];
+    int8_t* codes[2];
+    float* scales[2];
+    int64_t cap, start, n;
+    int H;
+};
+
+__device__ __forceinline__ uint32_t abs_bits(uint32_t bf16x2, int half) {
+    return half ? (bf16x2 & 0x7FFF0000u) : ((bf16x2 << 16) & 0x7FFF0000u);
+}
+
+__device__ __forceinline__ int quant1(float x, float s, bool live) {
+    if (!live) return 0;
+    const float r = rintf(__fdiv_rn(x, s));
+    return (int)fminf(fmaxf(r, -127.0f), 127.0f);
+}
+
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+    return (uint32_t)(a & 255) | ((uint32_t)(b & 255) << 8) | ((uint32_t)(c & 255) << 16) | ((uint32_t)(d & 255) << 24);
+}
+
+// One CTA per block of 64 tokens and head (blockIdx.x) and per K / V
+// (blockIdx.y).  A thread holds 8 consecutive channels of PASSES tokens in
+// registers between the maximum and the division, so x is read once.
+template <int D>
+__global__ void __launch_bounds__(kThreads) write_kernel(WriteArgs a) {
+    constexpr int kCols = D / 8;              // threads along the channels
+    constexpr int kRows = kThreads / kCols;   // tokens per pass
+    constexpr int kPasses = kBlock / kRows;
+    const int which = blockIdx.y;
+    const int h = (int)(blockIdx.x % (unsigned)a.H);
+    const int64_t b = a.start / kBlock + blockIdx.x / (unsigned)a.H;
+    const int64_t end = a.start + a.n;
+    const int col = threadIdx.x % kCols, row = threadIdx.x / kCols;
+    int8_t* codes = a.codes[which] + ((int64_t)h * a.cap + b * kBlock) * D + col * 8;
+    float* scale = a.scales[which] + (int64_t)h * (a.cap / kBlock) + b;
+
+    uint4 v[kPasses];
+    uint32_t top = 0;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+        const int64_t t = b * kBlock + row + p * kRows;
+        v[p] = make_uint4(0, 0, 0, 0);
+        if (t >= a.start && t < end)
+            v[p] = *reinterpret_cast<const uint4*>(a.x[which] + (t - a.start) * a.ld[which] + h * a.hs[which] + col * 8);
+    }
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+        const uint32_t w[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = max(top, max(abs_bits(w[e], 0), abs_bits(w[e], 1)));
+    }
+    __shared__ uint32_t tops[kThreads / 32];
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
+    const bool stays = a.start > b * kBlock;  // older tokens in this block
+    const float older = stays ? *scale : 0.0f;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) top = max(top, tops[w]);
+    // a NaN's quotient is a NaN: the order of the bit patterns still holds below
+    float s = __fdiv_rn(__uint_as_float(top), 127.0f);
+    if ((__float_as_uint(older) & 0x7FFFFFFFu) > (__float_as_uint(s) & 0x7FFFFFFFu)) s = older;
+    const bool live = s > 0.0f && s < __int_as_float(0x7F800000);
+    const bool grew = stays && __float_as_uint(s) != __float_as_uint(older);
+    const float ratio = grew && live ? __fdiv_rn(older, s) : 0.0f;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+        const int r = row + p * kRows;
+        const int64_t t = b * kBlock + r;
+        if (t >= end) continue;
+        uint2* dst = reinterpret_cast<uint2*>(codes + (int64_t)r * D);
+        if (t >= a.start) {
+            const uint32_t w[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
+            int c[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                c[2 * e] = quant1(bf16_lo(w[e]), s, live);
+                c[2 * e + 1] = quant1(bf16_hi(w[e]), s, live);
+            }
+            *dst = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+        } else if (grew) {
+            const uint2 old = *dst;
+            int c[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int8_t q = (int8_t)(((e < 4 ? old.x : old.y) >> (8 * (e & 3))) & 255u);
+                c[e] = (int)rintf(__fmul_rn((float)q, ratio));
+            }
+            *dst = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+        }
+    }
+    // `older` was read by every thread before the barrier above
+    if (threadIdx.x == 0) *scale = s;
+}
+
+struct ReadArgs {
+    const int8_t* codes[2];
+    const float* scales[2];
+    void* out[2];  // [n, H, D]
+    int64_t cap, start, n;
+    int H;
+};
+
+// One CTA per block of 64 tokens and head, per K / V; 8 codes a thread and pass.
+template <int D, bool F32>
+__global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
+    constexpr int kCols = D / 8;
+    constexpr int kRows = kThreads / kCols;
+    const int which = blockIdx.y;
+    const int h = (int)(blockIdx.x % (unsigned)a.H);
+    const int64_t b = a.start / kBlock + blockIdx.x / (unsigned)a.H;
+    const int col = threadIdx.x % kCols, row = threadIdx.x / kCols;
+    const int8_t* codes = a.codes[which] + ((int64_t)h * a.cap + b * kBlock) * D + col * 8;
+    const float s = a.scales[which][(int64_t)h * (a.cap / kBlock) + b];
+    uint2 v[kBlock / kRows];
+#pragma unroll
+    for (int p = 0; p < kBlock / kRows; ++p) {
+        const int64_t t = b * kBlock + row + p * kRows;
+        if (t >= a.start && t < a.start + a.n) v[p] = *reinterpret_cast<const uint2*>(codes + (row + p * kRows) * D);
+    }
+#pragma unroll
+    for (int p = 0; p < kBlock / kRows; ++p) {
+        const int64_t t = b * kBlock + row + p * kRows;
+        if (t < a.start || t >= a.start + a.n) continue;
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            f[e] = __fmul_rn((float)(int8_t)(((e < 4 ? v[p].x : v[p].y) >> (8 * (e & 3))) & 255u), s);
+        const int64_t at = ((t - a.start) * a.H + h) * D + col * 8;
+        if constexpr (F32) {
+            float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.out[which]) + at);
+            o[0] = make_float4(f[0], f[1], f[2], f[3]);
+            o[1] = make_float4(f[4], f[5], f[6], f[7]);
+        } else {
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out[which]) + at) =
+                make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                           pack_bf16x2(f[6], f[7]));
+        }
+    }
+}
+
+static int check_cache(const char* who, const void* kq, const void* vq, const void* ks, const void* vs, int64_t cap,
+                       int64_t start, int64_t n, int64_t H, int64_t D) {
+    H3B_REQUIRE(D == 64 || D == 128, "%s: head_dim=%lld must be 64 or 128", who, (long long)D);
+    H3B_REQUIRE(H > 0 && H <= 65535 && cap >= 0 && cap % kBlock == 0 && cap <= (1ll << 31),
+                "%s: heads=%lld and capacity=%lld (a multiple of %d) out of range", who, (long long)H, (long long)cap,
+                kBlock);
+    H3B_REQUIRE(start >= 0 && n >= 0 && start <= cap && n <= cap - start,
+                "%s: tokens [%lld, %lld) lie outside the capacity %lld", who, (long long)start, (long long)(start + n),
+                (long long)cap);
+    H3B_REQUIRE(n == 0 || (kq && vq && ks && vs), "%s: NULL cache pointer", who);
+    H3B_REQUIRE(aligned(kq, 16) && aligned(vq, 16) && aligned(ks, 4) && aligned(vs, 4),
+                "%s: codes must be 16-byte aligned", who);
+    const int64_t blocks = (start + n + kBlock - 1) / kBlock - start / kBlock;
+    H3B_REQUIRE(blocks * H < (1ll << 31), "%s: too many blocks in one call", who);
+    return H3B_OK;
+}
+
+}  // namespace kv8
+}  // namespace h3b
+
+using namespace h3b;
+
+extern "C" int h3b_kv8_write(const void* k, int64_t k_ld, int64_t k_hs, const void* v, int64_t v_ld, int64_t v_hs,
+                             int64_t start, int64_t n, int64_t H, int64_t D, int8_t* kq, int8_t* vq, float* ks,
+                             float* vs, int64_t cap, void* stream) {
+    if (int rc = kv8::check_cache("h3b_kv8_write", kq, vq, ks, vs, cap, start, n, H, D)) return rc;
+    if (n == 0) return H3B_OK;
+    H3B_REQUIRE(k && v && aligned(k, 16) && aligned(v, 16), "h3b_kv8_write: k / v NULL or not 16-byte aligned");
+    H3B_REQUIRE(k_ld % 8 == 0 && k_hs % 8 == 0 && v_ld % 8 == 0 && v_hs % 8 == 0,
+                "h3b_kv8_write: token and head strides must be multiples of 8 elements");
+    kv8::WriteArgs a{{static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v)},
+                     {k_ld, v_ld}, {k_hs, v_hs}, {kq, vq}, {ks, vs}, cap, start, n, (int)H};
+    const int64_t blocks = cdiv(start + n, kv8::kBlock) - start / kv8::kBlock;
+    const dim3 grid((unsigned)(blocks * H), 2);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (D == 128) kv8::write_kernel<128><<<grid, kv8::kThreads, 0, s>>>(a);
+    else kv8::write_kernel<64><<<grid, kv8::kThreads, 0, s>>>(a);
+    H3B_CUDA_TRY(cudaGetLastError());
+    return H3B_OK;
+}
+
+extern "C" int h3b_kv8_read(const int8_t* kq, const int8_t* vq, const float* ks, const float* vs, int64_t cap,
+                            int64_t start, int64_t n, int64_t H, int64_t D, void* k_out, void* v_out, int fp32,
+                            void* stream) {
+    if (int rc = kv8::check_cache("h3b_kv8_read", kq, vq, ks, vs, cap, start, n, H, D)) return rc;
+    if (n == 0) return H3B_OK;
+    H3B_REQUIRE(k_out && v_out && aligned(k_out, 16) && aligned(v_out, 16),
+                "h3b_kv8_read: outputs NULL or not 16-byte aligned");
+    kv8::ReadArgs a{{kq, vq}, {ks, vs}, {k_out, v_out}, cap, start, n, (int)H};
+    const int64_t blocks = cdiv(start + n, kv8::kBlock) - start / kv8::kBlock;
+    const dim3 grid((unsigned)(blocks * H), 2);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (D == 128 && fp32) kv8::read_kernel<128, true><<<grid, kv8::kThreads, 0, s>>>(a);
+    else if (D == 128) kv8::read_kernel<128, false><<<grid, kv8::kThreads, 0, s>>>(a);
+    else if (fp32) kv8::read_kernel<64, true><<<grid, kv8::kThreads, 0, s>>>(a);
+    else kv8::read_kernel<64, false><<<grid, kv8::kThreads, 0, s>>>(a);
+    H3B_CUDA_TRY(cudaGetLastError());
+    return H3B_OK;
+}

@@ -14,7 +14,7 @@ LIB_PATH = os.path.join(HERE, "libh3b.so")
 H3B_OK = 0
 STATUS_OK, STATUS_MBAR_TIMEOUT, STATUS_PEER_TIMEOUT, STATUS_BAD_INDEX = 0, 1, 2, 3
 STATUS_NAMES = {0: "ok", 1: "GEMM pipeline wait timed out", 2: "peer barrier timed out",
-                3: "modulation row index out of range"}
+                3: "modulation row or key block index out of range"}
 
 # (name, restype, argtypes)
 _P, _I64, _F32, _I32, _U32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_float, ctypes.c_int, ctypes.c_uint32
@@ -51,6 +51,14 @@ SIGNATURES = [
     ("h3b_peer_barrier", _I32, [_PP, _I32, _I32, _U32, _I64, _P]),
     ("h3b_a2a_fwd_p2p", _I32, [_I32, _PP, _I64, _PP, _I64, _I64, _I64, _I64, _I64, _I32, _P]),
     ("h3b_a2a_inv_quant", _I32, [_PP, _I64, _I64, _I64, _I64, _I32, _P, _P, _P]),
+    ("h3b_kv8_write", _I32, [_P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P]),
+    ("h3b_kv8_read", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I32, _P]),
+    ("h3b_kv8_attn", _I32, [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _F32, _P, _I64, _I64, _P]),
+    ("h3b_block_means", _I32, [_P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P]),
+    ("h3b_select_blocks_workspace", _I64, [_I64, _I64, _I64]),
+    ("h3b_select_blocks", _I32, [_P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),
+    ("h3b_block_sparse_attn", _I32, [_P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64,
+                                     _F32, _P, _I64, _I64, _P]),
     ("h3b_a2a_inv_p2p", _I32, [_P, _I64, _PP, ctypes.POINTER(ctypes.c_int64), _I64, _I64, _I64, _I32, _P]),
 ]
 

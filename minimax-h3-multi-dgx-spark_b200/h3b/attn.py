@@ -1,0 +1,253 @@
+"""Attention operators next to the block's SDPA: a key/value cache held in 8 bits, and block-sparse attention.
+
+  KV8Cache                 K/V of one sequence as int8 codes with an fp32 scale per 64 tokens and head
+    .write(k, v)             quantise new tokens into it;  .read() gives them back as bf16 / fp32
+  kv8_attention(q, cache)  softmax(scale * q K^T) V over the cached tokens
+  block_means(x, rows)     fp32 means of blocks of rows
+  select_blocks(qm, km, k) the k key blocks whose means have the largest products with a query block's mean
+  block_sparse_attention   softmax attention of each block of 128 query rows over its own blocks of 64 keys
+  sparse_attention         the three in a row
+
+They take the place of the attention between the qkv and the out projection of sp_attention
+(comfyui_nodes/minimax-h3-sp/minimax_sp/sp_forward.py:276-318), tensors being [tokens, heads, head_dim] with
+head_dim 64 or 128 as everywhere in h3b.  h3b.model uses them for a cached text context (SynthDiT.text_cache) and for
+sparse self-attention (DiTConfig.attn_topk).  Inputs may be strided over tokens and heads (multiples of 8 elements,
+16-byte aligned, unit stride over the head's channels); outputs are allocated with PyTorch's caching allocator on the
+input's device and the kernels run on its current stream.  No operator synchronises; under stream capture the sizes
+(a cache's length among them) are those of the capture.  There is no backward pass: the framework does not train.
+"""
+import contextlib
+
+import torch
+
+from ._lib import check, lib, ptr, require_cuda, stream_of
+from .trace import span
+
+BF16 = torch.bfloat16
+KEYS = 64    # tokens per scale of the cache, keys per sparse block
+QROWS = 128  # query rows that share a selection of key blocks
+
+
+def _on(t):
+    """Makes t's device the current one for the launches inside (nothing to do when it is)."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _rows(name, t, like=None):
+    """(token stride, head stride) of t [n, H, D] bf16 in elements; raises if the kernels cannot read it."""
+    if t.dtype != BF16 or t.dim() != 3:
+        raise ValueError(f"{name} must be a bf16 [tokens, heads, head_dim] tensor, got {t.dtype} {tuple(t.shape)}")
+    n, h, d = t.shape
+    if d not in (64, 128):
+        raise ValueError(f"{name}: head_dim {d} is not covered (64 or 128)")
+    if h == 0:
+        raise ValueError(f"{name}: no heads")
+    if like is not None and (t.shape[1:] != like.shape[1:] or t.device != like.device):
+        raise ValueError(f"{name} {tuple(t.shape)} on {t.device} does not go with {tuple(like.shape)} on {like.device}")
+    # the stride over a single token or head says nothing
+    ld = t.stride(0) if n > 1 else h * d
+    hs = t.stride(1) if h > 1 else d
+    if t.numel() and (t.stride(2) != 1 or ld % 8 or hs % 8 or ld <= 0 or hs <= 0 or t.data_ptr() % 16):
+        raise ValueError(f"{name}: strides {t.stride()} need a unit channel stride, positive token and head strides that "
+                         "are multiples of 8 elements, and a 16-byte aligned start; pass a contiguous copy")
+    return ld, hs
+
+
+def _scale(scale, d):
+    return d ** -0.5 if scale is None else float(scale)
+
+
+class KV8Cache:
+    """Keys and values of up to `capacity` tokens in 8 bits.
+
+    kq, vq: int8 codes [heads, capacity, head_dim]; ks, vs: fp32 scales [heads, capacity / 64], one per block of 64
+    tokens and head (capacity is rounded up to whole blocks).  `length` tokens are held; what lies behind them is
+    never read.  A token costs 2 * heads * (head_dim + 4 / 64) bytes, about half of bf16."""
+
+    def __init__(self, capacity, heads, head_dim, device="cuda"):
+        if capacity < 0 or heads <= 0 or head_dim not in (64, 128):
+            raise ValueError(f"KV8Cache: capacity {capacity}, heads {heads}, head_dim {head_dim} (64 or 128)")
+        cap = -(-int(capacity) // KEYS) * KEYS
+        kw = dict(device=device)
+        self._take(torch.empty((heads, cap, head_dim), dtype=torch.int8, **kw),
+                   torch.empty((heads, cap, head_dim), dtype=torch.int8, **kw),
+                   torch.empty((heads, cap // KEYS), dtype=torch.float32, **kw),
+                   torch.empty((heads, cap // KEYS), dtype=torch.float32, **kw), 0)
+
+    @classmethod
+    def wrap(cls, kq, vq, ks, vs, length):
+        """A cache over existing codes and scales (contiguous, laid out as above), of which `length` tokens are held."""
+        if kq.dim() != 3 or kq.dtype != torch.int8 or kq.shape[0] == 0 or kq.shape[2] not in (64, 128) or kq.shape[1] % KEYS:
+            raise ValueError("KV8Cache.wrap: kq must be int8 [heads, capacity, head_dim], capacity a multiple of "
+                             f"{KEYS} and head_dim 64 or 128; got {kq.dtype} {tuple(kq.shape)}")
+        scales = (kq.shape[0], kq.shape[1] // KEYS)
+        if vq.shape != kq.shape or vq.dtype != torch.int8 or any(
+                tuple(s.shape) != scales or s.dtype != torch.float32 for s in (ks, vs)):
+            raise ValueError(f"KV8Cache.wrap: vq must match kq, ks and vs must be fp32 {scales}")
+        if not all(t.is_contiguous() and t.device == kq.device and t.data_ptr() % 16 == 0 for t in (kq, vq, ks, vs)):
+            raise ValueError("KV8Cache.wrap: codes and scales must be contiguous, 16-byte aligned and on one device")
+        if not 0 <= length <= kq.shape[1]:
+            raise ValueError(f"KV8Cache.wrap: length {length} outside the capacity {kq.shape[1]}")
+        self = cls.__new__(cls)
+        self._take(kq, vq, ks, vs, int(length))
+        return self
+
+    def _take(self, kq, vq, ks, vs, length):
+        require_cuda(kq)
+        self.kq, self.vq, self.ks, self.vs, self.length = kq, vq, ks, vs, length
+
+    @property
+    def heads(self):
+        return self.kq.shape[0]
+
+    @property
+    def capacity(self):
+        return self.kq.shape[1]
+
+    @property
+    def head_dim(self):
+        return self.kq.shape[2]
+
+    def _goes_with(self, name, t):
+        if t.shape[1] != self.heads or t.shape[2] != self.head_dim or t.device != self.kq.device:
+            raise ValueError(f"{name} {tuple(t.shape)} on {t.device} does not go with a cache of {self.heads} heads of "
+                             f"{self.head_dim} on {self.kq.device}")
+
+    def write(self, k, v, start=None):
+        """Quantise k, v [n, heads, head_dim] (bf16) into tokens start .. start + n (start <= length, by default the
+        end); tokens that lay at and behind start are dropped.  A block's scale is its new tokens' absmax / 127, or
+        its former scale where older tokens stay in it and that is larger; staying codes are requantised when the
+        scale grows.  A NaN or infinity makes its block and head NaN.  Returns the cache."""
+        require_cuda(k, v)
+        start = self.length if start is None else int(start)
+        (kld, khs), (vld, vhs) = _rows("k", k), _rows("v", v, k)
+        self._goes_with("k", k)
+        n = k.shape[0]
+        if v.shape[0] != n:
+            raise ValueError(f"KV8Cache.write: {n} keys and {v.shape[0]} values")
+        if not 0 <= start <= self.length or start + n > self.capacity:
+            raise ValueError(f"KV8Cache.write: tokens {start} .. {start + n} do not follow the {self.length} held "
+                             f"within the capacity {self.capacity}")
+        H, D = self.heads, self.head_dim
+        if n:
+            with _on(k), span("kv8_write", 6 * n * H * D):
+                check(lib.h3b_kv8_write(ptr(k), kld, khs, ptr(v), vld, vhs, start, n, H, D, ptr(self.kq), ptr(self.vq),
+                                        ptr(self.ks), ptr(self.vs), self.capacity, stream_of(k)), "h3b_kv8_write")
+        self.length = start + n
+        return self
+
+    def read(self, start=0, stop=None, dtype=BF16):
+        """(k, v) [stop - start, heads, head_dim] of the held tokens: code * scale, rounded once more to bf16 unless
+        dtype is float32."""
+        stop = self.length if stop is None else int(stop)
+        start = int(start)
+        if not 0 <= start <= stop <= self.length:
+            raise ValueError(f"KV8Cache.read: tokens {start} .. {stop} are not among the {self.length} held")
+        if dtype not in (BF16, torch.float32):
+            raise ValueError(f"KV8Cache.read: dtype {dtype} is not covered (bfloat16 or float32)")
+        n, H, D = stop - start, self.heads, self.head_dim
+        k, v = (torch.empty((n, H, D), dtype=dtype, device=self.kq.device) for _ in "kv")
+        if n:
+            with _on(k), span("kv8_read", 2 * n * H * D * (1 + k.element_size())):
+                check(lib.h3b_kv8_read(ptr(self.kq), ptr(self.vq), ptr(self.ks), ptr(self.vs), self.capacity, start, n,
+                                       H, D, ptr(k), ptr(v), int(dtype == torch.float32), stream_of(k)), "h3b_kv8_read")
+        return k, v
+
+
+def kv8_attention(q, cache, scale=None):
+    """softmax(scale * q K^T) V of q [rows, heads, head_dim] over the tokens held in `cache` -> bf16 like q
+    (contiguous); scale defaults to head_dim ** -0.5.  An empty cache gives zeros."""
+    require_cuda(q)
+    ld, hs = _rows("q", q)
+    cache._goes_with("q", q)
+    sq, H, D = q.shape
+    o = torch.empty((sq, H, D), dtype=BF16, device=q.device)
+    if sq:
+        with _on(q), span("kv8_attn", 4.0 * sq * cache.length * H * D):
+            check(lib.h3b_kv8_attn(ptr(q), ld, hs, sq, H, D, ptr(cache.kq), ptr(cache.vq), ptr(cache.ks), ptr(cache.vs),
+                                   cache.capacity, cache.length, _scale(scale, D), ptr(o), H * D, D, stream_of(q)),
+                  "h3b_kv8_attn")
+    return o
+
+
+def block_means(x, rows=KEYS, out=None):
+    """fp32 [ceil(n / rows), heads, head_dim]: the mean of each block of `rows` (64 or 128) rows of x
+    [n, heads, head_dim] bf16, the last block's over the rows it has.  Summed in 64 bits and rounded once, so it does
+    not depend on an order.  out (optional, contiguous) takes the result: a program that appends keys keeps the means
+    and renews those of the blocks it touched, block_means(k[64 * b:], out=means[b:])."""
+    require_cuda(x)
+    ld, hs = _rows("x", x)
+    if rows not in (64, 128):
+        raise ValueError(f"block_means: rows {rows} is not covered (64 or 128)")
+    n, H, D = x.shape
+    shape = (-(-n // rows), H, D)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.float32, device=x.device)
+    elif tuple(out.shape) != shape or out.dtype != torch.float32 or not out.is_contiguous() or out.device != x.device:
+        raise ValueError(f"block_means: out must be contiguous fp32 {shape} on {x.device}")
+    if n:
+        with _on(x), span("block_means", 2 * x.numel()):
+            check(lib.h3b_block_means(ptr(x), ld, hs, n, H, D, rows, ptr(out), stream_of(x)), "h3b_block_means")
+    return out
+
+
+def select_blocks(qm, km, topk):
+    """int32 [heads, nq, min(topk, nk)]: for each head and row of qm [nq, heads, head_dim] (fp32 means of query
+    blocks) the rows of km [nk, heads, head_dim] with the largest products, ascending.  Products are summed in 64
+    bits; ties go to the lowest index, a NaN product ranks below every number."""
+    require_cuda(qm, km)
+    if qm.dim() != 3 or km.dim() != 3 or qm.shape[1:] != km.shape[1:] or qm.device != km.device:
+        raise ValueError(f"select_blocks: means {tuple(qm.shape)} and {tuple(km.shape)} do not go together")
+    if any(t.dtype != torch.float32 or not t.is_contiguous() for t in (qm, km)):
+        raise ValueError("select_blocks: means must be contiguous fp32 [blocks, heads, head_dim]")
+    (nq, H, D), nk = qm.shape, km.shape[0]
+    if D not in (64, 128) or H == 0:
+        raise ValueError(f"select_blocks: heads {H}, head_dim {D} (64 or 128)")
+    if topk < 0:
+        raise ValueError(f"select_blocks: topk {topk}")
+    topk = min(int(topk), nk)
+    blocks = torch.empty((H, nq, topk), dtype=torch.int32, device=qm.device)
+    if nq and topk:
+        ws = torch.empty(lib.h3b_select_blocks_workspace(nq, nk, H), dtype=torch.uint8, device=qm.device)
+        with _on(qm), span("select_blocks", 2.0 * nq * nk * H * D, launches=2):
+            check(lib.h3b_select_blocks(ptr(qm), ptr(km), nq, nk, H, D, topk, ptr(blocks), ptr(ws), ws.numel(),
+                                        stream_of(qm)), "h3b_select_blocks")
+    return blocks
+
+
+def block_sparse_attention(q, k, v, blocks, scale=None):
+    """softmax(scale * q K^T) V where query rows 128 i .. of head h see the keys of blocks[h, i, :] only, block b being
+    keys 64 b .. 64 b + 63 (those that exist).  q [rows, H, D], k / v [keys, H, D] bf16, blocks int32 [H,
+    ceil(rows / 128), n] contiguous; -1 stands for no block, a block named twice counts twice, and rows without a key
+    are zero.  An index outside -1 .. ceil(keys / 64) - 1 is skipped and recorded in the device status."""
+    require_cuda(q, k, v, blocks)
+    (qld, qhs), (kld, khs), (vld, vhs) = _rows("q", q), _rows("k", k, q), _rows("v", v, q)
+    sq, H, D = q.shape
+    nq = -(-sq // QROWS)
+    if v.shape[0] != k.shape[0]:
+        raise ValueError(f"block_sparse_attention: {k.shape[0]} keys and {v.shape[0]} values")
+    if blocks.dtype != torch.int32 or blocks.dim() != 3 or tuple(blocks.shape[:2]) != (H, nq) or \
+            not blocks.is_contiguous() or blocks.device != q.device:
+        raise ValueError(f"block_sparse_attention: blocks must be contiguous int32 [{H}, {nq}, n] on {q.device}, got "
+                         f"{blocks.dtype} {tuple(blocks.shape)}")
+    n = blocks.shape[2]
+    o = torch.empty((sq, H, D), dtype=BF16, device=q.device)
+    if sq:
+        with _on(q), span("sparse_attn", 4.0 * sq * n * KEYS * H * D):
+            check(lib.h3b_block_sparse_attn(ptr(q), qld, qhs, sq, H, D, ptr(k), kld, khs, ptr(v), vld, vhs, k.shape[0],
+                                            ptr(blocks), n, _scale(scale, D), ptr(o), H * D, D, stream_of(q)),
+                  "h3b_block_sparse_attn")
+    return o
+
+
+def sparse_attention(q, k, v, topk, scale=None, k_means=None, return_blocks=False):
+    """block_sparse_attention over the topk blocks of 64 keys that select_blocks finds for each block of 128 query
+    rows.  k_means: block_means(k) if the program keeps it.  With return_blocks, (o, blocks)."""
+    require_cuda(q, k, v)
+    if k_means is None:
+        k_means = block_means(k, KEYS)
+    elif k_means.shape[0] != -(-k.shape[0] // KEYS):
+        raise ValueError(f"sparse_attention: k_means has {k_means.shape[0]} blocks for {k.shape[0]} keys")
+    blocks = select_blocks(block_means(q, QROWS), k_means, topk)
+    o = block_sparse_attention(q, k, v, blocks, scale)
+    return (o, blocks) if return_blocks else o

@@ -28,7 +28,10 @@ copies with each step's compute.
 
 Weights are int8 with per-output-channel fp32 scales and bf16 biases, drawn
 from a seeded generator on the target device.  Attention stays PyTorch's
-scaled_dot_product_attention, as in the reference.
+scaled_dot_product_attention, as in the reference, unless DiTConfig.attn_topk
+selects block-sparse self-attention (h3b.attn.sparse_attention) or the text is
+given as a cache of its keys and values in 8 bits (SynthDiT.text_cache), which
+holds from one denoising step to the next.
 """
 import os
 from dataclasses import dataclass, field
@@ -36,7 +39,7 @@ from dataclasses import dataclass, field
 import torch
 import torch.nn.functional as F
 
-from . import fuse, sp
+from . import attn, fuse, sp
 from .linear import gelu_quant as _gelu_quant
 from .linear import gelu_tanh as _gelu
 from .linear import int8_mm_scaled as _mm8
@@ -88,6 +91,7 @@ class DiTConfig:
     n_blocks: int = 1
     text_len: int = 0  # > 0 enables the cross-attention branch
     qk_norm: bool = False  # per-head RMSNorm of q and k (attn.q_norm / k_norm), no RoPE
+    attn_topk: int = 0  # > 0: self-attention over this many selected blocks of 64 keys (0: dense SDPA)
 
 
 def make_params(cfg, block_index, seed, device, R=1):
@@ -140,6 +144,11 @@ def sdpa_heads(q, k, v):
     return sdpa(q, k, v).reshape(sq, h * dh)
 
 
+def self_sdpa(cfg, q, k, v):
+    """The self-attention core [S, h, Dh] -> [S, h, Dh]: SDPA, or block-sparse attention with cfg.attn_topk."""
+    return attn.sparse_attention(q, k, v, cfg.attn_topk) if cfg.attn_topk else sdpa(q, k, v)
+
+
 def self_attention(cfg, p, hq, ctx, overlap_groups=None):
     """hq: the quantised block input (codes, scales) of the modulated h.
 
@@ -158,7 +167,7 @@ def self_attention(cfg, p, hq, ctx, overlap_groups=None):
         # quantiser gathers its rows from every rank's output
         q, k, v = ctx.peer.gemm_fwd(hq[0], hq[1], p.qkv.w, p.qkv.ws, p.qkv.b, ctx,
                                     norm_w=p.qkn if cfg.qk_norm else None, norm_eps=cfg.eps)
-        return _lin_q(ctx.peer.inv_quant(sdpa(q, k, v), ctx), p.out)
+        return _lin_q(ctx.peer.inv_quant(self_sdpa(cfg, q, k, v), ctx), p.out)
     qkv = _lin_q(hq, p.qkv)  # [s, 3D]
     q = qkv[:, :D].view(s, H, Dh)
     k = qkv[:, D:2 * D].view(s, H, Dh)
@@ -166,24 +175,34 @@ def self_attention(cfg, p, hq, ctx, overlap_groups=None):
     if cfg.qk_norm:
         q = fuse.rms_norm(q.contiguous(), p.qkn[0], cfg.eps)
         k = fuse.rms_norm(k.contiguous(), p.qkn[1], cfg.eps)
+
+    def heads(q, k, v):  # [S, h, Dh] each -> [S, h*Dh]
+        return self_sdpa(cfg, q, k, v).reshape(q.shape[0], q.shape[1] * Dh)
+
     if not sharded:
-        return _lin(sdpa_heads(q, k, v), p.out)
+        return _lin(heads(q, k, v), p.out)
     if overlap:
-        return _lin(sp.sp_attention_overlap(q, k, v, ctx, sdpa_heads, n), p.out)
+        return _lin(sp.sp_attention_overlap(q, k, v, ctx, heads, n), p.out)
     q, k, v = sp.a2a_gather_qkv(q, k, v, ctx)  # [S, H/P, Dh] each
-    o = sdpa_heads(q, k, v)  # [S, (H/P)*Dh]
+    o = heads(q, k, v)  # [S, (H/P)*Dh]
     o = sp.a2a_scatter_seq_gather_heads(o, ctx)  # [s_local, D]
     return _lin(o, p.out)
 
 
-def cross_attention(cfg, p, hq, text):
-    s = hq[0].shape[0]
-    D, H, Dh = cfg.dim, cfg.heads, cfg.head_dim
-    q = _lin_q(hq, p.cq).view(s, H, Dh)
+def text_kv(cfg, p, text):
+    """The block's keys and values [t, H, Dh] of the text tokens [t, D]."""
     kv = _lin(text, p.ckv)
-    t = text.shape[0]
-    k = kv[:, :D].view(t, H, Dh)
-    v = kv[:, D:].view(t, H, Dh)
+    t, D = text.shape[0], cfg.dim
+    return kv[:, :D].view(t, cfg.heads, cfg.head_dim), kv[:, D:].view(t, cfg.heads, cfg.head_dim)
+
+
+def cross_attention(cfg, p, hq, text):
+    """text: the tokens [t, D], or an attn.KV8Cache of this block's keys and values of them."""
+    s = hq[0].shape[0]
+    q = _lin_q(hq, p.cq).view(s, cfg.heads, cfg.head_dim)
+    if isinstance(text, attn.KV8Cache):
+        return _lin(attn.kv8_attention(q, text).view(s, cfg.dim), p.cout)
+    k, v = text_kv(cfg, p, text)
     return _lin(sdpa_heads(q, k, v), p.cout)
 
 
@@ -249,9 +268,21 @@ class SynthDiT:
         self.device = torch.device(device)
         self.params = [make_params(cfg, i, seed, self.device) for i in range(cfg.n_blocks)]
 
-    def forward(self, x, ridx, ctx=None, text=None):
+    def text_cache(self, text):
+        """The text's keys and values of every block in 8 bits, to be passed as `text` to forward: computed once
+        for all denoising steps of a prompt instead of in each of them."""
+        caches = []
         for p in self.params:
-            x = block_forward(self.cfg, p, x, ridx, ctx, text)
+            k, v = text_kv(self.cfg, p, text)
+            caches.append(attn.KV8Cache(text.shape[0], self.cfg.heads, self.cfg.head_dim, self.device).write(k, v))
+        return caches
+
+    def forward(self, x, ridx, ctx=None, text=None):
+        """text: the text tokens [t, D], the list that text_cache gives, or None."""
+        if isinstance(text, (list, tuple)) and len(text) != len(self.params):
+            raise ValueError(f"SynthDiT.forward: {len(text)} text caches for {len(self.params)} blocks")
+        for i, p in enumerate(self.params):
+            x = block_forward(self.cfg, p, x, ridx, ctx, text[i] if isinstance(text, (list, tuple)) else text)
         return x
 
 

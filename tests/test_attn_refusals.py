@@ -1,0 +1,118 @@
+"""Refusals of the attention operators, without a GPU: the C entry points before any device work, and the Python checks."""
+import ctypes
+
+import pytest
+import torch
+
+import h3b
+from h3b._lib import lib
+
+P0 = ctypes.c_void_p(0)
+P16 = ctypes.c_void_p(4096)  # aligned, never dereferenced: each call is refused for another reason
+P2 = ctypes.c_void_p(4098)
+
+
+def refused(name, rc, word):
+    assert rc == -1, f"{name} returned {rc}"
+    msg = lib.h3b_last_error().decode()
+    assert name in msg and word in msg, msg
+
+
+def write(k=P16, kld=128, khs=128, start=0, n=1, H=1, D=128, kq=P16, cap=64):
+    return lib.h3b_kv8_write(k, kld, khs, P16, 128, 128, start, n, H, D, kq, P16, P16, P16, cap, P0)
+
+
+def test_write_refusals():
+    refused("h3b_kv8_write", write(D=96), "head_dim")
+    refused("h3b_kv8_write", write(H=0), "heads")
+    refused("h3b_kv8_write", write(cap=65), "capacity")
+    refused("h3b_kv8_write", write(start=64), "outside")
+    refused("h3b_kv8_write", write(start=-1), "outside")
+    refused("h3b_kv8_write", write(n=-1), "outside")
+    refused("h3b_kv8_write", write(start=1, n=2 ** 63 - 1), "outside")
+    refused("h3b_kv8_write", write(kq=P0), "NULL")
+    refused("h3b_kv8_write", write(k=P0), "NULL")
+    refused("h3b_kv8_write", write(k=P2), "aligned")
+    refused("h3b_kv8_write", write(kld=129), "strides")
+    assert write(n=0) == 0  # nothing to do, nothing launched
+
+
+def test_read_refusals():
+    def read(start=0, n=1, D=128, out=P16):
+        return lib.h3b_kv8_read(P16, P16, P16, P16, 64, start, n, 1, D, out, P16, 0, P0)
+    refused("h3b_kv8_read", read(D=32), "head_dim")
+    refused("h3b_kv8_read", read(start=60, n=5), "outside")
+    refused("h3b_kv8_read", read(out=P0), "NULL")
+    refused("h3b_kv8_read", read(out=P2), "aligned")
+    assert read(n=0) == 0
+
+
+def test_attention_refusals():
+    def cached(q=P16, qld=128, Sq=1, H=1, D=128, kq=P16, cap=64, length=64, o=P16):
+        return lib.h3b_kv8_attn(q, qld, 128, Sq, H, D, kq, P16, P16, P16, cap, length, 1.0, o, 128, 128, P0)
+    refused("h3b_kv8_attn", cached(length=65), "length")
+    refused("h3b_kv8_attn", cached(length=-1), "length")
+    refused("h3b_kv8_attn", cached(cap=100), "capacity")
+    refused("h3b_kv8_attn", cached(kq=P0), "NULL")
+    refused("h3b_kv8_attn", cached(H=0), "heads")
+    refused("h3b_kv8_attn", cached(D=256), "head_dim")
+    refused("h3b_kv8_attn", cached(q=P2), "aligned")
+    refused("h3b_kv8_attn", cached(o=P0), "NULL")
+    refused("h3b_kv8_attn", cached(qld=100), "strides")
+    refused("h3b_kv8_attn", cached(Sq=2 ** 40), "range")
+    assert cached(Sq=0) == 0
+
+    def sparse(k=P16, kld=128, Sk=64, blocks=P16, topk=1, D=128):
+        return lib.h3b_block_sparse_attn(P16, 128, 128, 1, 1, D, k, kld, 128, P16, 128, 128, Sk, blocks, topk, 1.0, P16,
+                                         128, 128, P0)
+    refused("h3b_block_sparse_attn", sparse(topk=-1), "topk")
+    refused("h3b_block_sparse_attn", sparse(blocks=P0), "blocks")
+    refused("h3b_block_sparse_attn", sparse(k=P2), "aligned")
+    refused("h3b_block_sparse_attn", sparse(kld=4), "strides")
+    refused("h3b_block_sparse_attn", sparse(Sk=-1), "range")
+    refused("h3b_block_sparse_attn", sparse(D=80), "head_dim")
+
+
+def test_selection_refusals():
+    def means(D=128, rows=64, x=P16, ld=128):
+        return lib.h3b_block_means(x, ld, 128, 5, 1, D, rows, P16, P0)
+    refused("h3b_block_means", means(D=16), "head_dim")
+    refused("h3b_block_means", means(rows=96), "rows")
+    refused("h3b_block_means", means(x=P0), "NULL")
+    refused("h3b_block_means", means(ld=12), "strides")
+
+    def select(nq=1, nk=4, topk=2, D=64, ws=P16, size=1 << 20):
+        return lib.h3b_select_blocks(P16, P16, nq, nk, 1, D, topk, P16, ws, size, P0)
+    refused("h3b_select_blocks", select(topk=5), "topk")
+    refused("h3b_select_blocks", select(topk=-1), "topk")
+    refused("h3b_select_blocks", select(D=72), "head_dim")
+    refused("h3b_select_blocks", select(ws=P0), "NULL")
+    refused("h3b_select_blocks", select(size=100), "workspace")
+    assert select(nq=0) == 0 and select(topk=0) == 0
+    assert lib.h3b_select_blocks_workspace(0, 5, 1) == 0
+    # one unit is 64 query blocks of a head; a workspace holds at least one, and at most 256 MiB beyond it
+    assert lib.h3b_select_blocks_workspace(65, 10, 3) == 2 * 3 * 64 * 10 * 8
+    assert lib.h3b_select_blocks_workspace(1, 1 << 20, 1) == 64 * (1 << 20) * 8
+
+
+def test_python_checks_on_the_cpu():
+    """No CPU path: CPU tensors raise TypeError, malformed caches ValueError."""
+    x = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(TypeError):
+        h3b.block_means(x)
+    with pytest.raises(TypeError):
+        h3b.sparse_attention(x, x, x, 1)
+    with pytest.raises(TypeError):
+        h3b.KV8Cache(64, 2, 64, device="cpu")
+    with pytest.raises(ValueError):
+        h3b.KV8Cache(64, 2, 96)
+    with pytest.raises(ValueError):
+        h3b.KV8Cache(-1, 2, 64)
+    kq, ks = torch.zeros(2, 128, 64, dtype=torch.int8), torch.zeros(2, 2)
+    for bad in ((kq.float(), kq, ks, ks, 0), (kq[:, :100], kq[:, :100], ks, ks, 0), (kq, kq[:1], ks, ks, 0),
+                (kq, kq, ks[:, :1], ks, 0), (kq, kq, ks, ks.double(), 0), (kq, kq, ks, ks, 129), (kq, kq, ks, ks, -1),
+                (kq.transpose(0, 1).contiguous().transpose(0, 1), kq, ks, ks, 0)):
+        with pytest.raises(ValueError):
+            h3b.KV8Cache.wrap(*bad)
+    with pytest.raises(TypeError):
+        h3b.KV8Cache.wrap(kq, kq, ks, ks, 0)
