@@ -272,12 +272,20 @@ H3B_API int h3b_kv8_read(const int8_t *kq, const int8_t *vq, const float *ks, co
                          int64_t start, int64_t n, int64_t H, int64_t D, void *k_out, void *v_out, int fp32,
                          void *stream);
 
+/* Workspace of the two attentions below in bytes, `segments` being the cache's
+ * ceil(length / 64) or the list's topk: with few query rows the keys are split
+ * over CTAs, whose parts meet there (0: none needed, NULL will do).  Calls that
+ * may overlap need workspaces of their own.  The reference's attention call is
+ * at sp_forward.py:276-318. */
+H3B_API int64_t h3b_attn_workspace(int64_t Sq, int64_t H, int64_t D, int64_t segments);
+
 /* o = softmax(scale * q K^T) V over the first `length` tokens of such a cache
  * (K = kq * ks, V = vq * vs); length 0 gives zeros.  Replaces the
  * scaled_dot_product_attention of sp_forward.py:276-318 where K and V are kept. */
 H3B_API int h3b_kv8_attn(const void *q, int64_t q_ld, int64_t q_hs, int64_t Sq, int64_t H, int64_t D,
                          const int8_t *kq, const int8_t *vq, const float *ks, const float *vs, int64_t cap,
-                         int64_t length, float scale, void *o, int64_t o_ld, int64_t o_hs, void *stream);
+                         int64_t length, float scale, void *o, int64_t o_ld, int64_t o_hs, void *workspace,
+                         int64_t workspace_bytes, void *stream);
 
 /* out[b, h, :] = mean of rows b * rows .. of x [S, H, D] bf16 (rows 64 or 128;
  * the last block over the rows it has) -> fp32 [ceil(S / rows), H, D], summed
@@ -304,7 +312,8 @@ H3B_API int h3b_select_blocks(const float *qm, const float *km, int64_t nq, int6
 H3B_API int h3b_block_sparse_attn(const void *q, int64_t q_ld, int64_t q_hs, int64_t Sq, int64_t H, int64_t D,
                                   const void *k, int64_t k_ld, int64_t k_hs, const void *v, int64_t v_ld,
                                   int64_t v_hs, int64_t Sk, const int32_t *blocks, int64_t topk, float scale,
-                                  void *o, int64_t o_ld, int64_t o_hs, void *stream);
+                                  void *o, int64_t o_ld, int64_t o_hs, void *workspace, int64_t workspace_bytes,
+                                  void *stream);
 
 /* ---- Ulysses all-to-all -------------------------------------------------- */
 

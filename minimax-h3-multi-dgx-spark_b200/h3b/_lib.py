@@ -53,12 +53,14 @@ SIGNATURES = [
     ("h3b_a2a_inv_quant", _I32, [_PP, _I64, _I64, _I64, _I64, _I32, _P, _P, _P]),
     ("h3b_kv8_write", _I32, [_P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P]),
     ("h3b_kv8_read", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I32, _P]),
-    ("h3b_kv8_attn", _I32, [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _F32, _P, _I64, _I64, _P]),
+    ("h3b_kv8_attn", _I32, [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _F32, _P, _I64, _I64, _P,
+                             _I64, _P]),
+    ("h3b_attn_workspace", _I64, [_I64, _I64, _I64, _I64]),
     ("h3b_block_means", _I32, [_P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P]),
     ("h3b_select_blocks_workspace", _I64, [_I64, _I64, _I64]),
     ("h3b_select_blocks", _I32, [_P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),
     ("h3b_block_sparse_attn", _I32, [_P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64,
-                                     _F32, _P, _I64, _I64, _P]),
+                                     _F32, _P, _I64, _I64, _P, _I64, _P]),
     ("h3b_a2a_inv_p2p", _I32, [_P, _I64, _PP, ctypes.POINTER(ctypes.c_int64), _I64, _I64, _I64, _I32, _P]),
 ]
 

@@ -49,7 +49,7 @@ def test_read_refusals():
 
 def test_attention_refusals():
     def cached(q=P16, qld=128, Sq=1, H=1, D=128, kq=P16, cap=64, length=64, o=P16):
-        return lib.h3b_kv8_attn(q, qld, 128, Sq, H, D, kq, P16, P16, P16, cap, length, 1.0, o, 128, 128, P0)
+        return lib.h3b_kv8_attn(q, qld, 128, Sq, H, D, kq, P16, P16, P16, cap, length, 1.0, o, 128, 128, P0, 0, P0)
     refused("h3b_kv8_attn", cached(length=65), "length")
     refused("h3b_kv8_attn", cached(length=-1), "length")
     refused("h3b_kv8_attn", cached(cap=100), "capacity")
@@ -60,11 +60,15 @@ def test_attention_refusals():
     refused("h3b_kv8_attn", cached(o=P0), "NULL")
     refused("h3b_kv8_attn", cached(qld=100), "strides")
     refused("h3b_kv8_attn", cached(Sq=2 ** 40), "range")
+    refused("h3b_kv8_attn", cached(qld=0), "strides")
+    refused("h3b_kv8_attn", cached(cap=4096, length=4096), "workspace")
+    assert lib.h3b_attn_workspace(1, 1, 128, 64) % (4 * 130) == 0 and lib.h3b_attn_workspace(1, 1, 128, 64) > 0
+    assert lib.h3b_attn_workspace(100000, 40, 128, 64) == 0 and lib.h3b_attn_workspace(0, 1, 128, 64) == 0
     assert cached(Sq=0) == 0
 
     def sparse(k=P16, kld=128, Sk=64, blocks=P16, topk=1, D=128):
         return lib.h3b_block_sparse_attn(P16, 128, 128, 1, 1, D, k, kld, 128, P16, 128, 128, Sk, blocks, topk, 1.0, P16,
-                                         128, 128, P0)
+                                         128, 128, P0, 0, P0)
     refused("h3b_block_sparse_attn", sparse(topk=-1), "topk")
     refused("h3b_block_sparse_attn", sparse(blocks=P0), "blocks")
     refused("h3b_block_sparse_attn", sparse(k=P2), "aligned")
