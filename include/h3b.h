@@ -272,12 +272,14 @@ H3B_API int h3b_kv8_read(const int8_t *kq, const int8_t *vq, const float *ks, co
                          int64_t start, int64_t n, int64_t H, int64_t D, void *k_out, void *v_out, int fp32,
                          void *stream);
 
-/* Workspace of the two attentions below in bytes, `segments` being the cache's
- * ceil(length / 64) or the list's topk: with few query rows the keys are split
- * over CTAs, whose parts meet there (0: none needed, NULL will do).  Calls that
- * may overlap need workspaces of their own.  The reference's attention call is
- * at sp_forward.py:276-318. */
-H3B_API int64_t h3b_attn_workspace(int64_t Sq, int64_t H, int64_t D, int64_t segments);
+/* Workspace of the two attentions below in bytes (256-byte aligned; 0: none
+ * needed, NULL will do): h3b_kv8_attn with `cache` set and segments =
+ * ceil(length / 64), h3b_block_sparse_attn with cache 0 and segments = topk.
+ * With few row tiles the keys are split over CTAs, whose parts meet there; with
+ * many, a cache's codes are widened to bf16 there once (at most 256 MiB of
+ * heads, or one head, at a time).  Calls that may overlap need workspaces of
+ * their own.  The reference's attention call is at sp_forward.py:276-318. */
+H3B_API int64_t h3b_attn_workspace(int cache, int64_t Sq, int64_t H, int64_t D, int64_t segments);
 
 /* o = softmax(scale * q K^T) V over the first `length` tokens of such a cache
  * (K = kq * ks, V = vq * vs); length 0 gives zeros.  Replaces the

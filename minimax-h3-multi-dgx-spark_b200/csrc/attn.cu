@@ -16,6 +16,7 @@ struct Args {
     int64_t o_ld, o_hs;
     int64_t Sq, keys;
     int H;
+    int h0;  // first head of the launch
     float scale;
     // 8-bit cache
     const int8_t* codes[2];
@@ -27,7 +28,7 @@ struct Args {
     const int32_t* blocks;
     int topk;
     int64_t nq;  // query tiles of 128 rows
-    // parts of a split: O [parts, H, Sq, D], (reference maximum, sum) [parts, H, Sq, 2]
+    // parts of a split: O [parts, H, Sq, D], (reference maximum, sum) [parts, H, Sq, 2], H of the launch
     float* part_o;
     float* part_ml;
     int* status;
@@ -116,23 +117,22 @@ __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32
 __device__ __forceinline__ void tmem_ready(uint32_t (&r)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" : H3B_R16(r, 0), H3B_R16(r, 16)::"memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
         "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
-        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-        "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -179,12 +179,18 @@ __device__ __forceinline__ uint32_t codes_to_bf16x2(uint32_t x, uint32_t sel) {
     return *reinterpret_cast<const uint32_t*>(&d);
 }
 
+// Where the keys and values of a step come from.
+enum Source {
+    kBlocks,  // selected blocks of bf16 tensors, by TMA
+    kWide,    // the cache's codes widened to bf16 beforehand, by TMA
+    kCodes,   // the cache's codes, widened by four warps of the CTA
+};
+
 // Warps 0-3: softmax, one row a thread; warp 4: the MMAs; after them the
-// operand warps: 4 that turn codes into bf16 tiles (cache), or one that issues
-// the TMA loads of the selected blocks.
-template <bool CACHE>
+// operand warps, one that issues TMA loads or four that widen codes.
+template <Source SRC>
 constexpr int tile_threads() {
-    return CACHE ? 288 : 192;
+    return SRC == kCodes ? 288 : 192;
 }
 
 // One step's segments: 64 keys each, `n` of them valid, starting at token `at`.
@@ -193,19 +199,112 @@ struct Seg {
     int n;
 };
 
-template <bool CACHE>
+template <Source SRC>
 __device__ __forceinline__ Seg segment(const Args& a, const int32_t* list, int64_t index, int64_t count) {
     if (index >= count) return Seg{a.keys, 0};
     int64_t b = index;
-    if constexpr (!CACHE) {
+    if constexpr (SRC == kBlocks) {
         b = __ldg(list + index);
         if (b < 0 || b * kSeg >= a.keys) return Seg{a.keys, 0};
     }
     return Seg{b * kSeg, (int)min((int64_t)kSeg, a.keys - b * kSeg)};
 }
 
-template <int D, bool CACHE>
-__global__ void __launch_bounds__(tile_threads<CACHE>(), 2)
+struct Row {
+    float m, l;  // reference maximum (in powers of two) and sum of 2^(x - m)
+};
+
+// One step of a row: S (128 columns at tS) -> P (bf16, 64 columns at tS), with
+// the running maximum and sum.  n, sk, sv: per segment of 64 keys its valid
+// keys, the factor of its scores (softmax scale, log2 e and, for codes, the
+// block's scale) and of its values.  TAIL: some keys are not valid.
+template <int D, Source SRC, bool TAIL>
+__device__ __forceinline__ void softmax_step(Row& st, uint32_t tS, uint32_t tO, bool later, const int (&n)[2],
+                                             const float (&sk)[2], const float (&sv)[2]) {
+    // with four widening warps in the CTA a thread has too few registers to
+    // hold the 128 scores from the maximum to the exponential: they are read twice
+    constexpr bool kHold = SRC != kCodes;
+    uint32_t r[4][32];
+    float mx[2][4];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mx[s][c] = -INFINITY;
+    if constexpr (kHold) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32_async(tS + c * 32, r[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ready(r[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        if constexpr (!kHold) {
+            tmem_ld32_async(tS + c * 32, r[0]);
+            tmem_ready(r[0]);
+        }
+        const uint32_t(&x)[32] = r[kHold ? c : 0];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            if (TAIL && (c & 1) * 32 + e >= n[c / 2]) continue;
+            mx[c / 2][e & 3] = fmaxf(mx[c / 2][e & 3], __uint_as_float(x[e]));
+        }
+    }
+    float top = -INFINITY;  // the step's largest score
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+        if (!TAIL || n[s] > 0)
+            top = fmaxf(top, fmaxf(fmaxf(mx[s][0], mx[s][1]), fmaxf(mx[s][2], mx[s][3])) * sk[s]);
+    const bool moves = top > st.m + kSlack || (st.m == -INFINITY && top > st.m);
+    if (__any_sync(0xFFFFFFFFu, moves)) {
+        // (this step's S has been waited for, and with it every product before: O stands still)
+        const float keep = moves ? ex2(st.m - top) : 1.0f;
+        if (moves) st.m = top;
+        st.l *= keep;
+        if (later) {
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+                uint32_t o[16];
+                tmem_ld16(tO + c * 16, o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                tmem_st16(tO + c * 16, o);
+            }
+        }
+    }
+    const float ref = st.m == -INFINITY ? 0.0f : st.m;
+    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        if constexpr (!kHold) {
+            tmem_ld32_async(tS + c * 32, r[0]);
+            tmem_ready(r[0]);
+        }
+        const uint32_t(&y)[32] = r[kHold ? c : 0];
+        const float k = sk[c / 2], v = sv[c / 2];
+        uint32_t p[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            float2 x = fma2(make_float2(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1])), make_float2(k, k),
+                            make_float2(-ref, -ref));
+            if constexpr (TAIL) {  // behind the product: a scale of zero must not bring a masked key back as NaN
+                if ((c & 1) * 32 + 2 * e >= n[c / 2]) x.x = -INFINITY;
+                if ((c & 1) * 32 + 2 * e + 1 >= n[c / 2]) x.y = -INFINITY;
+            }
+            x.x = ex2(x.x);
+            x.y = ex2(x.y);
+            sum[e & 1] = add2(sum[e & 1], x);
+            // p is rounded to bf16 for the second product (its sum is not): a relative 2^-8 at most a key
+            if constexpr (SRC != kBlocks) x = mul2(x, make_float2(v, v));
+            p[e] = pack_bf16x2(x.x, x.y);
+        }
+        tmem_st16(tS + c * 16, p);
+    }
+    sum[0] = add2(sum[0], sum[1]);
+    st.l += sum[0].x + sum[0].y;
+}
+
+template <int D, Source SRC>
+__global__ void __launch_bounds__(tile_threads<SRC>(), 2)
     tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, Args a) {
     using L = Smem<D>;
@@ -222,9 +321,10 @@ __global__ void __launch_bounds__(tile_threads<CACHE>(), 2)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // query tiles first: CTAs that run together share a head's keys in L2
     const int64_t qt = blockIdx.x % (unsigned)a.nq;
-    const int h = (int)(blockIdx.x / (unsigned)a.nq);
-    const int32_t* list = CACHE ? nullptr : a.blocks + ((int64_t)h * a.nq + qt) * a.topk;
-    const int64_t segs = CACHE ? (a.keys + kSeg - 1) / kSeg : a.topk;
+    const int hl = (int)(blockIdx.x / (unsigned)a.nq);  // head within the launch
+    const int h = a.h0 + hl;
+    const int32_t* list = SRC == kBlocks ? a.blocks + ((int64_t)h * a.nq + qt) * a.topk : nullptr;
+    const int64_t segs = SRC == kBlocks ? a.topk : (a.keys + kSeg - 1) / kSeg;
     const int64_t steps_all = (segs + 1) / 2;
     const int64_t step0 = steps_all * blockIdx.y / gridDim.y;
     const int steps = (int)(steps_all * (blockIdx.y + 1) / gridDim.y - step0);
@@ -236,8 +336,8 @@ __global__ void __launch_bounds__(tile_threads<CACHE>(), 2)
     }
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
-        mbar_init(k_full, CACHE ? 4 : 1);
-        mbar_init(v_full, CACHE ? 4 : 1);
+        mbar_init(k_full, SRC == kCodes ? 4 : 1);
+        mbar_init(v_full, SRC == kCodes ? 4 : 1);
         mbar_init(k_empty, 1);
         mbar_init(v_empty, 1);
         mbar_init(s_full, 1);
@@ -304,7 +404,7 @@ __global__ void __launch_bounds__(tile_threads<CACHE>(), 2)
         }
         __syncwarp();
     } else if (warp > 4) {
-        if constexpr (CACHE) {
+        if constexpr (SRC == kCodes) {
             // ---------------- codes -> bf16 tiles
             constexpr int kLanes = D / 16;          // threads along a token's channels, 16 codes each
             constexpr int kRows = 128 / kLanes;     // tokens per pass
@@ -362,8 +462,8 @@ __global__ void __launch_bounds__(tile_threads<CACHE>(), 2)
                 if (i + 1 < steps) fetch(1, i + 1);
             }
         } else if (lane == 0) {
-            // ---------------- TMA loads of the selected blocks; what is not there (a gap in the list, keys
-            // behind the last) lies outside the tensor and arrives as zeros
+            // ---------------- TMA loads; what is not there (a gap in the list, keys behind the last) lies
+            // outside the tensor and arrives as zeros
             bool ok = true;
             int k_armed = 0, v_armed = 0;
             for (int i = 0; ok && i < steps; ++i) {
@@ -372,8 +472,8 @@ __global__ void __launch_bounds__(tile_threads<CACHE>(), 2)
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     const int64_t index = 2 * (step0 + i) + s;
-                    at[s] = (int)segment<CACHE>(a, list, index, segs).at;
-                    if (index < segs) {
+                    at[s] = (int)segment<SRC>(a, list, index, segs).at;
+                    if (SRC == kBlocks && index < segs) {
                         const int64_t b = __ldg(list + index);
                         if (b < -1 || b * kSeg >= a.keys) report(a.status, H3B_STATUS_BAD_INDEX);
                     }
@@ -390,7 +490,8 @@ __global__ void __launch_bounds__(tile_threads<CACHE>(), 2)
                     for (int s = 0; s < 2; ++s)
 #pragma unroll
                         for (int c = 0; c < L::kHalves; ++c)
-                            tma_load_3d((w ? sV : sK) + c * 16384 + s * 8192, w ? &tmV : &tmK, full, c * 64, h, at[s]);
+                            tma_load_3d((w ? sV : sK) + c * 16384 + s * 8192, w ? &tmV : &tmK, full, c * 64,
+                                        SRC == kBlocks ? h : hl, at[s]);
                     ++(w ? v_armed : k_armed);
                 }
             }
@@ -407,98 +508,39 @@ __global__ void __launch_bounds__(tile_threads<CACHE>(), 2)
         const uint32_t at = (uint32_t)(warp * 32) << 16;
         const int64_t row = qt * kQRows + threadIdx.x;
         const float scale2 = fabsf(a.scale) * kLog2e;
-        float m = -INFINITY, l = 0.0f;
+        Row st{-INFINITY, 0.0f};
         bool ok = true;
         for (int i = 0; i < steps; ++i) {
             int n[2];
             float sk[2], sv[2];
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                const Seg g = segment<CACHE>(a, list, 2 * (step0 + i) + s, segs);
+                const Seg g = segment<SRC>(a, list, 2 * (step0 + i) + s, segs);
                 n[s] = g.n;
                 sk[s] = scale2;
                 sv[s] = 1.0f;
-                if (CACHE && g.n > 0) {
+                if (SRC != kBlocks && g.n > 0) {
                     sk[s] = scale2 * __ldg(a.scales[0] + (int64_t)h * (a.cap / kSeg) + g.at / kSeg);
                     sv[s] = __ldg(a.scales[1] + (int64_t)h * (a.cap / kSeg) + g.at / kSeg);
                 }
             }
-            const bool whole = n[0] + n[1] == kTileKeys;
             if (!(ok = mbar_wait(s_full, (uint32_t)i & 1u, abort_flag, a.status, kWaitNs))) break;
             tc_fence_after();
-            // the step's largest score, scaled to powers of two
-            float top = -INFINITY;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                float mx = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t r[32];
-                    tmem_ld32_async(tS + at + s * 64 + c * 32, r);
-                    tmem_ready(r);
-                    if (!whole) {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (c * 32 + e >= n[s]) r[e] = 0xFF800000u;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(r[e]));
-                }
-                if (n[s] > 0) top = fmaxf(top, mx * sk[s]);
-            }
-            const bool moves = top > m + kSlack || (m == -INFINITY && top > m);
-            if (__any_sync(0xFFFFFFFFu, moves)) {
-                // (everything up to this step's S has been waited for, so O stands still)
-                const float keep = moves ? ex2(m - top) : 1.0f;
-                if (moves) m = top;
-                l *= keep;
-                if (i > 0) {
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t r[32];
-                        tmem_ld32_async(tO + at + c * 32, r);
-                        tmem_ready(r);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * keep);
-                        tmem_st32(tO + at + c * 32, r);
-                    }
-                }
-            }
-            const float ref = m == -INFINITY ? 0.0f : m;
-            float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int s = c / 2;
-                uint32_t r[32], p[16];
-                tmem_ld32_async(tS + at + c * 32, r);
-                tmem_ready(r);
-                const float2 k2 = make_float2(sk[s], sk[s]), m2 = make_float2(-ref, -ref), v2 = make_float2(sv[s], sv[s]);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float2 x = fma2(make_float2(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), k2, m2);
-                    if (!whole) {  // behind the product: a scale of zero must not bring a masked key back as NaN
-                        if ((c & 1) * 32 + 2 * e >= n[s]) x.x = -INFINITY;
-                        if ((c & 1) * 32 + 2 * e + 1 >= n[s]) x.y = -INFINITY;
-                    }
-                    x.x = ex2(x.x);
-                    x.y = ex2(x.y);
-                    sum = add2(sum, x);
-                    if constexpr (CACHE) x = mul2(x, v2);
-                    p[e] = pack_bf16x2(x.x, x.y);
-                }
-                tmem_st16(tS + at + c * 16, p);
-            }
-            l += sum.x + sum.y;
+            if (n[0] + n[1] == kTileKeys)
+                softmax_step<D, SRC, false>(st, tS + at, tO + at, i > 0, n, sk, sv);
+            else
+                softmax_step<D, SRC, true>(st, tS + at, tO + at, i > 0, n, sk, sv);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full);
         }
+        const float m = st.m, l = st.l;
         if (ok && steps > 0) ok = mbar_wait(o_full, 0, abort_flag, a.status, kWaitNs);
         tc_fence_after();
         if (ok && gridDim.y > 1) {
             // a part of the keys: O, its reference maximum and sum go to the join
-            const int64_t part = ((int64_t)blockIdx.y * a.H + h) * a.Sq + row;
+            const int64_t part = (int64_t)blockIdx.y * gridDim.x / a.nq * a.Sq + (int64_t)hl * a.Sq + row;
             if (row < a.Sq) {
                 a.part_ml[2 * part] = m;
                 a.part_ml[2 * part + 1] = l;
@@ -564,13 +606,13 @@ __global__ void __launch_bounds__(tile_threads<CACHE>(), 2)
 
 // Join of the parts of a split: o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.  One warp a row.
 template <int D>
-__global__ void __launch_bounds__(128) join_kernel(Args a, int parts) {
+__global__ void __launch_bounds__(128) join_kernel(Args a, int heads, int parts) {
     const int lane = threadIdx.x & 31;
     const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (id >= a.Sq * a.H) return;
-    const int h = (int)(id / a.Sq);
+    const int64_t step = a.Sq * heads;
+    if (id >= step) return;
+    const int h = a.h0 + (int)(id / a.Sq);
     const int64_t row = id % a.Sq;
-    const int64_t step = a.Sq * a.H;
     float m = -INFINITY;
     for (int s = lane; s < parts; s += 32) m = fmaxf(m, a.part_ml[2 * (s * step + id)]);
 #pragma unroll
@@ -588,6 +630,30 @@ __global__ void __launch_bounds__(128) join_kernel(Args a, int parts) {
     uint16_t* dst = a.o + row * a.o_ld + h * a.o_hs + lane * (D / 32);
 #pragma unroll
     for (int e = 0; e < D / 32; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(o[e] * inv, o[e + 1] * inv);
+}
+
+// Codes of some heads (each `per` pieces of 16 from `stride` pieces apart) -> bf16, K or V by blockIdx.y.
+__global__ void __launch_bounds__(256) widen_kernel(const int8_t* __restrict__ kq, const int8_t* __restrict__ vq,
+                                                    int64_t stride, int64_t per, int64_t pieces,
+                                                    uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
+    const uint4* src = reinterpret_cast<const uint4*>(blockIdx.y ? vq : kq);
+    uint4* dst = reinterpret_cast<uint4*>(blockIdx.y ? v : k);
+    uint4 x[4];
+    const int64_t first = (int64_t)blockIdx.x * 1024 + threadIdx.x;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const int64_t i = first + p * 256;
+        if (i < pieces) x[p] = __ldg(src + i / per * stride + i % per);
+    }
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const int64_t i = first + p * 256;
+        if (i >= pieces) break;
+        dst[2 * i] = make_uint4(codes_to_bf16x2(x[p].x, 0x4140), codes_to_bf16x2(x[p].x, 0x4342),
+                                codes_to_bf16x2(x[p].y, 0x4140), codes_to_bf16x2(x[p].y, 0x4342));
+        dst[2 * i + 1] = make_uint4(codes_to_bf16x2(x[p].z, 0x4140), codes_to_bf16x2(x[p].z, 0x4342),
+                                    codes_to_bf16x2(x[p].w, 0x4140), codes_to_bf16x2(x[p].w, 0x4342));
+    }
 }
 
 // [tokens, heads, D] bf16 as boxes of `rows` tokens x 64 channels of a head.
@@ -616,43 +682,87 @@ static int sm_count() {
     return cached;
 }
 
-// Parts of the keys that the work of a row tile is split into: as many as fill
-// the two CTAs of every SM once, of at least `least` steps each.
-static int64_t split(int64_t tiles, int64_t steps, int64_t least) {
-    const int64_t room = 2 * sm_count() / (tiles > 0 ? tiles : 1);
-    const int64_t most = steps / least;
-    int64_t n = room < most ? room : most;
-    return n < 1 ? 1 : n;
+// Parts that the keys of every row tile are split into.  All CTAs take about as
+// long, so the time is the number of rounds of two CTAs an SM times a part's
+// steps plus what a CTA spends besides (about two steps); a join costs about
+// two more.
+static int64_t parts_of(int64_t tiles, int64_t steps) {
+    const int64_t room = 2 * sm_count();
+    int64_t best = 1, best_cost = 0;
+    for (int64_t n = 1; n <= 64 && (n == 1 || n * 2 <= steps); ++n) {
+        const int64_t cost = cdiv(tiles * n, room) * (cdiv(steps, n) + 2) + (n > 1 ? 2 : 0);
+        if (n == 1 || cost < best_cost) best = n, best_cost = cost;
+    }
+    return best;
 }
 
-static int64_t parts_of(int64_t Sq, int64_t H, int64_t segs) {
-    return split(cdiv(Sq, kQRows) * H, (segs + 1) / 2, 2);
+struct Plan {
+    bool wide;          // the cache's codes are widened beforehand
+    int64_t heads;      // heads a launch (and of the widened copy)
+    int64_t parts;      // of the keys
+    int64_t join_at, bytes;  // in the workspace
+};
+
+// From this many row tiles on a head's codes are widened once instead of by every CTA.
+constexpr int64_t kWideTiles = 4;
+constexpr int64_t kWideBytes = 256ll << 20;  // of widened heads at a time (one head at least)
+
+static Plan plan(bool cache, int64_t Sq, int64_t H, int64_t D, int64_t segs) {
+    Plan p{};
+    const int64_t nq = cdiv(Sq, kQRows);
+    p.wide = cache && nq >= kWideTiles && segs > 0;
+    const int64_t head = 2 * segs * kSeg * D * 2;
+    p.heads = H;
+    if (p.wide && H * head > kWideBytes) p.heads = kWideBytes / head > 0 ? kWideBytes / head : 1;
+    p.parts = parts_of(nq * p.heads, cdiv(segs, 2));
+    p.join_at = p.wide ? p.heads * head : 0;
+    p.bytes = p.join_at + (p.parts > 1 ? p.parts * p.heads * Sq * (D + 2) * 4 : 0);
+    return p;
 }
 
-static int64_t workspace(int64_t Sq, int64_t H, int64_t D, int64_t segs) {
-    const int64_t n = parts_of(Sq, H, segs);
-    return n > 1 ? n * Sq * H * (D + 2) * 4 : 0;
-}
-
-template <int D, bool CACHE>
-static int launch_tiles(Args& a, int parts, cudaStream_t s) {
+template <int D, Source SRC>
+static int launch_tiles(Args a, int64_t heads, int64_t parts, const uint16_t* const (&kv)[2], const int64_t (&ld)[2],
+                        const int64_t (&hs)[2], cudaStream_t s) {
     CUtensorMap q{}, k{}, v{}, o{};
     if (int rc = make_map(&q, a.q, a.Sq, a.H, D, a.q_ld, a.q_hs, kQRows)) return rc;
     if (int rc = make_map(&o, a.o, a.Sq, a.H, D, a.o_ld, a.o_hs, kQRows)) return rc;
-    if (!CACHE && a.keys > 0) {
-        if (int rc = make_map(&k, a.kv[0], a.keys, a.H, D, a.kv_ld[0], a.kv_hs[0], kSeg)) return rc;
-        if (int rc = make_map(&v, a.kv[1], a.keys, a.H, D, a.kv_ld[1], a.kv_hs[1], kSeg)) return rc;
+    if (SRC != kCodes && a.keys > 0) {
+        const int n = SRC == kBlocks ? a.H : (int)heads;
+        if (int rc = make_map(&k, kv[0], a.keys, n, D, ld[0], hs[0], kSeg)) return rc;
+        if (int rc = make_map(&v, kv[1], a.keys, n, D, ld[1], hs[1], kSeg)) return rc;
     }
-    H3B_CUDA_TRY(cudaFuncSetAttribute(tile_kernel<D, CACHE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes));
-    const dim3 grid((unsigned)(a.nq * a.H), (unsigned)parts);
-    tile_kernel<D, CACHE><<<grid, tile_threads<CACHE>(), Smem<D>::kBytes, s>>>(q, k, v, o, a);
-    if (parts > 1) join_kernel<D><<<(unsigned)cdiv(a.Sq * a.H, 4), 128, 0, s>>>(a, parts);
+    H3B_CUDA_TRY(cudaFuncSetAttribute(tile_kernel<D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes));
+    const dim3 grid((unsigned)(a.nq * heads), (unsigned)parts);
+    tile_kernel<D, SRC><<<grid, tile_threads<SRC>(), Smem<D>::kBytes, s>>>(q, k, v, o, a);
+    if (parts > 1) join_kernel<D><<<(unsigned)cdiv(a.Sq * heads, 4), 128, 0, s>>>(a, (int)heads, (int)parts);
     H3B_CUDA_TRY(cudaGetLastError());
     return H3B_OK;
 }
 
-template <bool CACHE>
-static int launch(const char* who, Args& a, int64_t D, int64_t segs, void* ws, int64_t ws_bytes, cudaStream_t s) {
+template <int D>
+static int launch_all(Args& a, bool cache, const Plan& p, int64_t segs, char* ws, cudaStream_t s) {
+    a.part_o = reinterpret_cast<float*>(ws + p.join_at);
+    a.part_ml = a.part_o + (p.parts > 1 ? p.parts * p.heads * a.Sq * D : 0);
+    if (!cache) return launch_tiles<D, kBlocks>(a, a.H, p.parts, a.kv, a.kv_ld, a.kv_hs, s);
+    if (!p.wide) return launch_tiles<D, kCodes>(a, a.H, p.parts, a.kv, a.kv_ld, a.kv_hs, s);
+    const int64_t rows = segs * kSeg;
+    uint16_t* const k = reinterpret_cast<uint16_t*>(ws);
+    for (int64_t h = 0; h < a.H; h += p.heads) {
+        const int64_t n = a.H - h < p.heads ? a.H - h : p.heads;
+        uint16_t* const v = k + n * rows * D;
+        const int64_t pieces = n * rows * D / 16;
+        widen_kernel<<<dim3((unsigned)cdiv(pieces, 4 * 256), 2), 256, 0, s>>>(
+            a.codes[0] + h * a.cap * D, a.codes[1] + h * a.cap * D, a.cap * D / 16, rows * D / 16, pieces, k, v);
+        a.h0 = (int)h;
+        const int64_t ld[2] = {D, D}, hs[2] = {rows * D, rows * D};
+        const uint16_t* const kv[2] = {k, v};
+        if (int rc = launch_tiles<D, kWide>(a, n, p.parts, kv, ld, hs, s)) return rc;
+    }
+    return H3B_OK;
+}
+
+static int launch(const char* who, bool cache, Args& a, int64_t D, int64_t segs, void* ws, int64_t ws_bytes,
+                  cudaStream_t s) {
     H3B_REQUIRE(D == 64 || D == 128, "%s: head_dim=%lld must be 64 or 128", who, (long long)D);
     H3B_REQUIRE(a.Sq >= 0 && a.keys >= 0 && a.H > 0 && a.H <= 65535 && a.Sq < (1ll << 31) - 128 &&
                     a.keys < (1ll << 31) - 128,
@@ -663,17 +773,15 @@ static int launch(const char* who, Args& a, int64_t D, int64_t segs, void* ws, i
                     a.o_ld % 8 == 0 && a.o_hs % 8 == 0,
                 "%s: strides must be positive multiples of 8 elements", who);
     a.nq = cdiv(a.Sq, kQRows);
-    H3B_REQUIRE(a.nq * a.H < (1ll << 31), "%s: too many row tiles", who);
-    const int64_t parts = parts_of(a.Sq, a.H, segs);
-    const int64_t need = workspace(a.Sq, a.H, D, segs);
-    H3B_REQUIRE(need == 0 || (ws && aligned(ws, 16) && ws_bytes >= need), "%s: workspace of %lld bytes, %lld needed", who,
-                (long long)ws_bytes, (long long)need);
-    a.part_o = static_cast<float*>(ws);
-    a.part_ml = static_cast<float*>(ws) + (parts > 1 ? parts * a.Sq * a.H * D : 0);
+    H3B_REQUIRE(a.nq * a.H < (1ll << 31) && a.Sq * a.H < (1ll << 33), "%s: too many row tiles", who);
+    const Plan p = plan(cache, a.Sq, a.H, D, segs);
+    H3B_REQUIRE(p.bytes == 0 || (ws && aligned(ws, 256) && ws_bytes >= p.bytes),
+                "%s: workspace of %lld bytes (256-byte aligned), %lld needed", who, (long long)ws_bytes, (long long)p.bytes);
     DeviceStatus ds;
     if (int rc = device_status(&ds)) return rc;
     a.status = ds.word;
-    return D == 128 ? launch_tiles<128, CACHE>(a, (int)parts, s) : launch_tiles<64, CACHE>(a, (int)parts, s);
+    return D == 128 ? launch_all<128>(a, cache, p, segs, static_cast<char*>(ws), s)
+                    : launch_all<64>(a, cache, p, segs, static_cast<char*>(ws), s);
 }
 
 }  // namespace attn
@@ -681,9 +789,9 @@ static int launch(const char* who, Args& a, int64_t D, int64_t segs, void* ws, i
 
 using namespace h3b;
 
-extern "C" int64_t h3b_attn_workspace(int64_t Sq, int64_t H, int64_t D, int64_t segments) {
+extern "C" int64_t h3b_attn_workspace(int cache, int64_t Sq, int64_t H, int64_t D, int64_t segments) {
     if (Sq <= 0 || H <= 0 || segments <= 0 || (D != 64 && D != 128)) return 0;
-    return attn::workspace(Sq, H, D, segments);
+    return attn::plan(cache != 0, Sq, H, D, segments).bytes;
 }
 
 extern "C" int h3b_kv8_attn(const void* q, int64_t q_ld, int64_t q_hs, int64_t Sq, int64_t H, int64_t D,
@@ -703,7 +811,7 @@ extern "C" int h3b_kv8_attn(const void* q, int64_t q_ld, int64_t q_hs, int64_t S
     a.o_ld = o_ld, a.o_hs = o_hs;
     a.Sq = Sq, a.keys = length, a.H = (int)H, a.scale = scale;
     a.codes[0] = kq, a.codes[1] = vq, a.scales[0] = ks, a.scales[1] = vs, a.cap = cap;
-    return attn::launch<true>("h3b_kv8_attn", a, D, cdiv(length, attn::kSeg), workspace, workspace_bytes,
+    return attn::launch("h3b_kv8_attn", true, a, D, cdiv(length, attn::kSeg), workspace, workspace_bytes,
                               static_cast<cudaStream_t>(stream));
 }
 
@@ -729,6 +837,6 @@ extern "C" int h3b_block_sparse_attn(const void* q, int64_t q_ld, int64_t q_hs, 
     a.kv[0] = static_cast<const uint16_t*>(k), a.kv[1] = static_cast<const uint16_t*>(v);
     a.kv_ld[0] = k_ld, a.kv_hs[0] = k_hs, a.kv_ld[1] = v_ld, a.kv_hs[1] = v_hs;
     a.blocks = blocks, a.topk = (int)topk;
-    return attn::launch<false>("h3b_block_sparse_attn", a, D, topk, workspace, workspace_bytes,
+    return attn::launch("h3b_block_sparse_attn", false, a, D, topk, workspace, workspace_bytes,
                                static_cast<cudaStream_t>(stream));
 }

@@ -55,7 +55,7 @@ SIGNATURES = [
     ("h3b_kv8_read", _I32, [_P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I32, _P]),
     ("h3b_kv8_attn", _I32, [_P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64, _F32, _P, _I64, _I64, _P,
                              _I64, _P]),
-    ("h3b_attn_workspace", _I64, [_I64, _I64, _I64, _I64]),
+    ("h3b_attn_workspace", _I64, [_I32, _I64, _I64, _I64, _I64]),
     ("h3b_block_means", _I32, [_P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P]),
     ("h3b_select_blocks_workspace", _I64, [_I64, _I64, _I64]),
     ("h3b_select_blocks", _I32, [_P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),

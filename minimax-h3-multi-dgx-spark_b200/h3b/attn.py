@@ -57,9 +57,9 @@ def _scale(scale, d):
     return d ** -0.5 if scale is None else float(scale)
 
 
-def _workspace(q, segments):
-    """Where the parts of a split over the keys meet: (tensor or None, bytes)."""
-    n = lib.h3b_attn_workspace(q.shape[0], q.shape[1], q.shape[2], segments)
+def _workspace(cache, q, segments):
+    """(tensor or None, bytes): where the parts of a split over the keys meet and a cache's codes are widened."""
+    n = lib.h3b_attn_workspace(cache, q.shape[0], q.shape[1], q.shape[2], segments)
     return (torch.empty(n, dtype=torch.uint8, device=q.device) if n else None), n
 
 
@@ -169,7 +169,7 @@ def kv8_attention(q, cache, scale=None):
     sq, H, D = q.shape
     o = torch.empty((sq, H, D), dtype=BF16, device=q.device)
     if sq:
-        ws, nbytes = _workspace(q, -(-cache.length // KEYS))
+        ws, nbytes = _workspace(1, q, -(-cache.length // KEYS))
         with _on(q), span("kv8_attn", 4.0 * sq * cache.length * H * D):
             check(lib.h3b_kv8_attn(ptr(q), ld, hs, sq, H, D, ptr(cache.kq), ptr(cache.vq), ptr(cache.ks), ptr(cache.vs),
                                    cache.capacity, cache.length, _scale(scale, D), ptr(o), H * D, D,
@@ -240,7 +240,7 @@ def block_sparse_attention(q, k, v, blocks, scale=None):
     n = blocks.shape[2]
     o = torch.empty((sq, H, D), dtype=BF16, device=q.device)
     if sq:
-        ws, nbytes = _workspace(q, n)
+        ws, nbytes = _workspace(0, q, n)
         with _on(q), span("sparse_attn", 4.0 * sq * n * KEYS * H * D):
             check(lib.h3b_block_sparse_attn(ptr(q), qld, qhs, sq, H, D, ptr(k), kld, khs, ptr(v), vld, vhs, k.shape[0],
                                             ptr(blocks), n, _scale(scale, D), ptr(o), H * D, D,
