@@ -28,6 +28,9 @@ struct Args {
     const int32_t* blocks;
     int topk;
     int64_t nq;  // query tiles of 128 rows
+    int64_t segs;   // segments of 64 keys
+    uint32_t items;  // pairs of tiles of the launch
+    int heads, parts;  // heads of the launch, parts of the keys
     // parts of a split: O [parts, H, Sq, D], (reference maximum, sum) [parts, H, Sq, 2], H of the launch
     float* part_o;
     float* part_ml;
@@ -35,10 +38,19 @@ struct Args {
 };
 
 // ---------------------------------------------------------------------------
-// Tile kernel: 128 query rows of one head per CTA, 128 keys per step.
+// Pair kernel: a persistent CTA per SM works on two tiles of 128 query rows at a
+// time, 64 keys a step each.
+//
+// A step of a tile is a chain: S = Q K^T (tensor cores), softmax of S (its own
+// four warps, one row a thread), O += P V (tensor cores).  TMEM holds, per tile,
+// O and two S of 64 columns (P takes the place of its S), so that the next
+// step's S is there when a softmax ends, and neither the softmax warps nor the
+// tensor cores wait for a chain to go round.  (One S of 128 columns a tile, the
+// other form that fits in TMEM, left the tensor cores idle more than half of the
+// time: the chain of a step took 3700 clocks, of which 1024 are products.)
 
-constexpr int kTileKeys = 128;  // keys per step: two segments
-constexpr int kTmemCols = 256;  // S / P: columns 0-127, O: columns 128 ..
+constexpr int kTmemCols = 512;     // S of tile t at 128 t (+ 64 for odd steps), O at 256 + 128 t
+constexpr int kPairThreads = 352;  // 2 x 4 softmax warps, an MMA warp for each tile, the TMA warp
 constexpr uint64_t kWaitNs = 1000ull * 1000 * 1000;
 constexpr float kLog2e = 1.4426950408889634f;
 // A row's reference maximum moves when a score exceeds it by 2^8: until then p
@@ -48,11 +60,14 @@ constexpr float kSlack = 8.0f;
 
 template <int D>
 struct Smem {
-    static constexpr int kHalves = D / 64;                 // 128-byte column halves of a row
-    static constexpr int kTile = kHalves * 128 * 128;      // 128 rows x D bf16
-    static constexpr int kQ = 0, kK = kTile, kV = 2 * kTile, kBars = 3 * kTile;
-    // at most two CTAs fit beside one another on an SM, as their TMEM does
-    static constexpr int kBytes = (3 * kTile + 256 > 80 * 1024) ? 3 * kTile + 256 : 80 * 1024;
+    static constexpr int kHalves = D / 64;             // 128-byte column halves of a row
+    static constexpr int kTile = kHalves * 128 * 128;  // 128 rows x D bf16: Q, O
+    static constexpr int kSegHalf = kSeg * 128;        // 64 keys of a half
+    static constexpr int kSegTile = kHalves * kSegHalf;
+    // K and V arrive in groups: the keys of a step with the values of the step two before it
+    static constexpr int kGroup = 2 * kSegTile, kGroups = 4;
+    static constexpr int kQ = 0, kKV = 2 * kTile, kO = kKV + kGroups * kGroup, kBars = kO + kTile;
+    static constexpr int kBytes = kBars + 256;
 };
 
 // kind::f16 instruction descriptor: D fp32 (bits 4-5 = 1), A and B bf16 (7-9 = 1,
@@ -62,26 +77,36 @@ constexpr uint32_t idesc(int n, bool b_mn_major) {
            (8u << 24);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
+// Shared-memory descriptors are built inside the MMA's asm from a low word (start
+// address >> 4, leading byte offset >> 4 at bit 16), which stepping along the
+// operand only adds to, and a constant high word: stride byte offset 1024 (8 rows
+// of 128 bytes), version 1, 128-byte swizzle.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+// K-major: rows of 64 channels; the leading byte offset is not used.
+__device__ __forceinline__ uint32_t desc_k(const void* p) { return ((smem_u32(p) >> 4) & 0x3FFFu) | (1u << 16); }
+// MN-major (V): rows are keys, the contraction, of 64 channels each; the next 64
+// channels lie kSeg rows on, the leading byte offset.
+__device__ __forceinline__ uint32_t desc_mn(const void* p) {
+    return ((smem_u32(p) >> 4) & 0x3FFFu) | (((uint32_t)kSeg * 128u >> 4) << 16);
+}
+
+// D (TMEM) [+]= A (shared memory) B^T
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(id), "r"(acc), "n"(kDescHi)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool acc) {
+// the same with A in TMEM
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "mov.b64 y, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(id), "r"(acc), "n"(kDescHi)
         : "memory");
-}
-// MN-major operand with 128-byte swizzle: rows are keys (the contraction), 64
-// channels each; the next 64 channels lie a half tile (16 KB) on (leading byte
-// offset), the next 8 keys 1024 bytes on (stride byte offset).
-__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
@@ -168,6 +193,13 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     return d;
 }
 
+// max of three, NaN if one of them is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // Two int8 codes (bytes `sel` picks, zero-extended to 16 bits) -> bf16x2, exactly:
 // in [128, 256) a bf16 steps by 1, so 0x4300 | low 7 bits is 128 + them, and
 // 0x4300 | sign bit is 128, or 256 for a negative code.
@@ -179,89 +211,82 @@ __device__ __forceinline__ uint32_t codes_to_bf16x2(uint32_t x, uint32_t sel) {
     return *reinterpret_cast<const uint32_t*>(&d);
 }
 
-// Where the keys and values of a step come from.
+// Where a tile's keys and values come from.
 enum Source {
-    kBlocks,  // selected blocks of bf16 tensors, by TMA
-    kWide,    // the cache's codes widened to bf16 beforehand, by TMA
-    kCodes,   // the cache's codes, widened by four warps of the CTA
+    kBlocks,  // selected blocks of bf16 tensors, each tile its own
+    kWide,    // the cache's codes widened to bf16 beforehand, the same for both tiles of a pair
 };
 
-// Warps 0-3: softmax, one row a thread; warp 4: the MMAs; after them the
-// operand warps, one that issues TMA loads or four that widen codes.
-template <Source SRC>
-constexpr int tile_threads() {
-    return SRC == kCodes ? 288 : 192;
-}
-
-// One step's segments: 64 keys each, `n` of them valid, starting at token `at`.
+// One step's segment: 64 keys, `n` of them valid, starting at token `at`.
 struct Seg {
-    int64_t at;
-    int n;
+    int at, n;
 };
-
-template <Source SRC>
-__device__ __forceinline__ Seg segment(const Args& a, const int32_t* list, int64_t index, int64_t count) {
-    if (index >= count) return Seg{a.keys, 0};
-    int64_t b = index;
-    if constexpr (SRC == kBlocks) {
-        b = __ldg(list + index);
-        if (b < 0 || b * kSeg >= a.keys) return Seg{a.keys, 0};
-    }
-    return Seg{b * kSeg, (int)min((int64_t)kSeg, a.keys - b * kSeg)};
-}
 
 struct Row {
     float m, l;  // reference maximum (in powers of two) and sum of 2^(x - m)
 };
 
-// One step of a row: S (128 columns at tS) -> P (bf16, 64 columns at tS), with
-// the running maximum and sum.  n, sk, sv: per segment of 64 keys its valid
-// keys, the factor of its scores (softmax scale, log2 e and, for codes, the
-// block's scale) and of its values.  TAIL: some keys are not valid.
-template <int D, Source SRC, bool TAIL>
-__device__ __forceinline__ void softmax_step(Row& st, uint32_t tS, uint32_t tO, bool later, const int (&n)[2],
-                                             const float (&sk)[2], const float (&sv)[2]) {
-    // with four widening warps in the CTA a thread has too few registers to
-    // hold the 128 scores from the maximum to the exponential: they are read twice
-    constexpr bool kHold = SRC != kCodes;
-    uint32_t r[4][32];
-    float mx[2][4];
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) mx[s][c] = -INFINITY;
-    if constexpr (kHold) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32_async(tS + c * 32, r[c]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ready(r[c]);
-    }
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        if constexpr (!kHold) {
-            tmem_ld32_async(tS + c * 32, r[0]);
-            tmem_ready(r[0]);
-        }
-        const uint32_t(&x)[32] = r[kHold ? c : 0];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-            if (TAIL && (c & 1) * 32 + e >= n[c / 2]) continue;
-            mx[c / 2][e & 3] = fmaxf(mx[c / 2][e & 3], __uint_as_float(x[e]));
+// Bounded wait for a phase.  False if the wait gave up or another role has.  (A
+// barrier is shared memory, which the products' operands keep busy: a look at
+// one takes some 250 clocks here, so what can be is asked for together.)
+__device__ __forceinline__ bool await(uint64_t* bar, uint32_t phase, volatile int* abort_flag, int* status) {
+    uint64_t t0 = 0;
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(phase & 1u)
+            : "memory");
+        if (ok) return true;
+        if (*abort_flag) return false;
+        const uint64_t now = globaltimer_ns();
+        if (!t0) t0 = now;
+        if (now - t0 > kWaitNs) {
+            *abort_flag = 1;
+            report(status, H3B_STATUS_MBAR_TIMEOUT);
+            return false;
         }
     }
-    float top = -INFINITY;  // the step's largest score
+}
+
+// One step of a row: S (64 columns at tS) -> P (bf16, 32 columns at tS), with the
+// running maximum and sum.  n: valid keys; sk, sv: factors of the scores (softmax
+// scale, log2 e and, for codes, the block's scale) and of the values.  TAIL: not
+// all keys are valid.  product_done() waits for the product before, after which O
+// may be rescaled; first: there is none.
+template <int D, Source SRC, bool TAIL, typename Wait>
+__device__ __forceinline__ void softmax_step(Row& st, uint32_t tS, uint32_t tO, bool first, int n, float sk, float sv,
+                                             const Wait& product_done) {
+    uint32_t r[2][32];
+    tmem_ld32_async(tS, r[0]);
+    tmem_ld32_async(tS + 32, r[1]);
+    tmem_ready(r[0]);
+    tmem_ready(r[1]);
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
-        if (!TAIL || n[s] > 0)
-            top = fmaxf(top, fmaxf(fmaxf(mx[s][0], mx[s][1]), fmaxf(mx[s][2], mx[s][3])) * sk[s]);
+    for (int e = 0; e < 64; e += 2) {
+        float y[2] = {__uint_as_float(r[e / 32][e % 32]), __uint_as_float(r[e / 32][e % 32 + 1])};
+        if constexpr (TAIL) {
+            if (e >= n) y[0] = -INFINITY;
+            if (e + 1 >= n) y[1] = -INFINITY;
+        }
+        mx[(e >> 1) & 3] = max3_nan(mx[(e >> 1) & 3], y[0], y[1]);
+    }
+    // the step's largest score, NaN if one is
+    float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * sk;
+    if (TAIL && n == 0) top = -INFINITY;
     const bool moves = top > st.m + kSlack || (st.m == -INFINITY && top > st.m);
     if (__any_sync(0xFFFFFFFFu, moves)) {
-        // (this step's S has been waited for, and with it every product before: O stands still)
         const float keep = moves ? ex2(st.m - top) : 1.0f;
         if (moves) st.m = top;
         st.l *= keep;
-        if (later) {
-#pragma unroll
+        if (!first) {
+            product_done();
+            tc_fence_after();
+#pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
                 uint32_t o[16];
                 tmem_ld16(tO + c * 16, o);
@@ -271,30 +296,26 @@ __device__ __forceinline__ void softmax_step(Row& st, uint32_t tS, uint32_t tO, 
             }
         }
     }
+    // a NaN or +infinity among the scores makes the row NaN, through its sum
+    if (!(top < INFINITY)) st.l = __int_as_float(0x7FC00000);
     const float ref = st.m == -INFINITY ? 0.0f : st.m;
     float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        if constexpr (!kHold) {
-            tmem_ld32_async(tS + c * 32, r[0]);
-            tmem_ready(r[0]);
-        }
-        const uint32_t(&y)[32] = r[kHold ? c : 0];
-        const float k = sk[c / 2], v = sv[c / 2];
+    for (int c = 0; c < 2; ++c) {
         uint32_t p[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            float2 x = fma2(make_float2(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1])), make_float2(k, k),
-                            make_float2(-ref, -ref));
+            float2 x = fma2(make_float2(__uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1])),
+                            make_float2(sk, sk), make_float2(-ref, -ref));
             if constexpr (TAIL) {  // behind the product: a scale of zero must not bring a masked key back as NaN
-                if ((c & 1) * 32 + 2 * e >= n[c / 2]) x.x = -INFINITY;
-                if ((c & 1) * 32 + 2 * e + 1 >= n[c / 2]) x.y = -INFINITY;
+                if (c * 32 + 2 * e >= n) x.x = -INFINITY;
+                if (c * 32 + 2 * e + 1 >= n) x.y = -INFINITY;
             }
             x.x = ex2(x.x);
             x.y = ex2(x.y);
             sum[e & 1] = add2(sum[e & 1], x);
             // p is rounded to bf16 for the second product (its sum is not): a relative 2^-8 at most a key
-            if constexpr (SRC != kBlocks) x = mul2(x, make_float2(v, v));
+            if constexpr (SRC == kWide) x = mul2(x, make_float2(sv, sv));
             p[e] = pack_bf16x2(x.x, x.y);
         }
         tmem_st16(tS + c * 16, p);
@@ -303,50 +324,107 @@ __device__ __forceinline__ void softmax_step(Row& st, uint32_t tS, uint32_t tO, 
     st.l += sum[0].x + sum[0].y;
 }
 
+// An item is a pair of tiles and a part of the keys; its tiles have the same steps.
+struct Item {
+    int part, step0, steps;
+    bool both;        // tile 1 is there
+    uint32_t pair;
+};
+
+template <Source SRC>
+__device__ __forceinline__ uint32_t pairs_of(const Args& a) {
+    return SRC == kWide ? ((uint32_t)a.nq + 1) / 2 * (uint32_t)a.heads : ((uint32_t)a.nq * (uint32_t)a.heads + 1) / 2;
+}
+
+template <Source SRC>
+__device__ __forceinline__ Item item_of(const Args& a, uint32_t item) {
+    Item it;
+    const uint32_t pairs = pairs_of<SRC>(a), all = (uint32_t)a.segs;
+    it.part = (int)(item / pairs);
+    it.pair = item - it.part * pairs;
+    it.step0 = (int)(all * it.part / (uint32_t)a.parts);
+    it.steps = (int)(all * (it.part + 1) / (uint32_t)a.parts) - it.step0;  // one at least: there are no more parts than steps
+    if constexpr (SRC == kWide) {
+        const uint32_t row = ((uint32_t)a.nq + 1) / 2;
+        it.both = 2 * (it.pair % row) + 1 < (uint32_t)a.nq;
+    } else {
+        it.both = 2 * it.pair + 1 < (uint32_t)a.nq * (uint32_t)a.heads;
+    }
+    return it;
+}
+
+// Head (within the launch) and query tile of tile t of a pair: query tiles first,
+// so that CTAs that run together share a head's keys in L2.
+struct Where {
+    int h, qt;
+};
+template <Source SRC>
+__device__ __forceinline__ Where where(const Args& a, uint32_t pair, int t) {
+    if constexpr (SRC == kWide) {
+        const uint32_t row = ((uint32_t)a.nq + 1) / 2, h = pair / row;
+        return Where{(int)h, (int)(2 * (pair - h * row)) + t};
+    } else {
+        const uint32_t id = 2 * pair + t, h = id / (uint32_t)a.nq;
+        return Where{(int)h, (int)(id - h * (uint32_t)a.nq)};
+    }
+}
+
+// Segment `index` of a tile's keys; list: the tile's blocks (kBlocks).  n < 0: an index out of range.
+template <Source SRC>
+__device__ __forceinline__ Seg segment(const Args& a, const int32_t* list, int index) {
+    if (index >= a.segs) return Seg{(int)a.keys, 0};
+    int64_t b = index;
+    if constexpr (SRC == kBlocks) {
+        b = __ldg(list + index);
+        if (b < 0 || b * kSeg >= a.keys) return Seg{(int)a.keys, b == -1 ? 0 : -1};
+    }
+    return Seg{(int)(b * kSeg), (int)min((int64_t)kSeg, a.keys - b * kSeg)};
+}
+template <Source SRC>
+__device__ __forceinline__ const int32_t* list_of(const Args& a, const Where& w) {
+    return SRC == kBlocks ? a.blocks + ((int64_t)(a.h0 + w.h) * a.nq + w.qt) * a.topk : nullptr;
+}
+
 template <int D, Source SRC>
-__global__ void __launch_bounds__(tile_threads<SRC>(), 2)
-    tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, Args a) {
+__global__ void __launch_bounds__(kPairThreads, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
+                const __grid_constant__ Args a) {
     using L = Smem<D>;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t* sQ = smem + L::kQ;
-    uint8_t* sK = smem + L::kK;
-    uint8_t* sV = smem + L::kV;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
-    uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 2, *v_full = bars + 3, *v_empty = bars + 4,
-             *s_full = bars + 5, *p_full = bars + 6, *o_full = bars + 7;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 8);
+    uint64_t *kv_full = bars, *kv_empty = bars + 4,  // of the groups
+        *s_full = bars + 8, *p_full = bars + 12,     // [tile][buffer]
+        *q_full = bars + 16, *q_empty = bars + 18, *pv_done = bars + 20, *out_full = bars + 22, *drain = bars + 24,  // [tile]
+        *out_free = bars + 26;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 27);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // query tiles first: CTAs that run together share a head's keys in L2
-    const int64_t qt = blockIdx.x % (unsigned)a.nq;
-    const int hl = (int)(blockIdx.x / (unsigned)a.nq);  // head within the launch
-    const int h = a.h0 + hl;
-    const int32_t* list = SRC == kBlocks ? a.blocks + ((int64_t)h * a.nq + qt) * a.topk : nullptr;
-    const int64_t segs = SRC == kBlocks ? a.topk : (a.keys + kSeg - 1) / kSeg;
-    const int64_t steps_all = (segs + 1) / 2;
-    const int64_t step0 = steps_all * blockIdx.y / gridDim.y;
-    const int steps = (int)(steps_all * (blockIdx.y + 1) / gridDim.y - step0);
-
     // the swizzled tiles need the 1024-byte alignment that this declaration asks for
     if (smem_u32(smem) & 1023u) {
         if (threadIdx.x == 0) report(a.status, H3B_STATUS_MBAR_TIMEOUT);
         return;
     }
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 1);
-        mbar_init(k_full, SRC == kCodes ? 4 : 1);
-        mbar_init(v_full, SRC == kCodes ? 4 : 1);
-        mbar_init(k_empty, 1);
-        mbar_init(v_empty, 1);
-        mbar_init(s_full, 1);
-        mbar_init(p_full, 4);
-        mbar_init(o_full, 1);
+        for (int j = 0; j < 4; ++j) {
+            mbar_init(kv_full + j, 1);
+            mbar_init(kv_empty + j, SRC == kWide ? 2 : 1);  // (kWide: both tiles read a group)
+            mbar_init(s_full + j, 1);
+            mbar_init(p_full + j, 4);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(q_full + t, 1);
+            mbar_init(q_empty + t, 1);
+            mbar_init(pv_done + t, 1);
+            mbar_init(out_full + t, 4);
+            mbar_init(drain + t, 1);
+        }
+        mbar_init(out_free, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 4) {
+    if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                      "r"(kTmemCols)
                      : "memory");
@@ -356,251 +434,278 @@ __global__ void __launch_bounds__(tile_threads<SRC>(), 2)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const uint32_t tS = tmem, tO = tmem + 128u;
 
-    if (warp == 4) {
-        // ---------------- MMA issuer (and the load of Q)
-        if (lane == 0 && steps > 0) {
-            mbar_expect_tx(q_full, L::kTile);
-#pragma unroll
-            for (int c = 0; c < L::kHalves; ++c)
-                tma_load_3d(sQ + c * 16384, &tmQ, q_full, c * 64, h, (int)(qt * kQRows));
-            const uint32_t id_s = idesc(kTileKeys, false) | (a.scale < 0.0f ? 1u << 13 : 0u);
+    // Groups of loads are numbered through the CTA's steps: group g brings the keys of step g and the values of step
+    // g - 2, for one tile (kBlocks, two places each) or for both (kWide, four places).
+    if (warp == 8 || warp == 9) {
+        // ---------------- MMA issuer of tile t
+        if (lane == 0) {
+            const int t = warp - 8;
+            const uint32_t id_s = idesc(kSeg, false) | (a.scale < 0.0f ? 1u << 13 : 0u);
             const uint32_t id_o = idesc(D, true);
-            const uint32_t q0 = smem_u32(sQ), k0 = smem_u32(sK), v0 = smem_u32(sV);
-            bool ok = mbar_wait(q_full, 0, abort_flag, a.status, kWaitNs);
-            for (int i = 0; ok && i <= steps; ++i) {
-                if (i > 0) {
-                    // O += P V of the step before
-                    const uint32_t ph = (uint32_t)(i - 1) & 1u;
-                    ok = mbar_wait(v_full, ph, abort_flag, a.status, kWaitNs) &&
-                         mbar_wait(p_full, ph, abort_flag, a.status, kWaitNs);
-                    if (!ok) break;
+            const uint32_t q0 = desc_k(smem + L::kQ + t * L::kTile), k0 = desc_k(smem + L::kKV),
+                           v0 = desc_mn(smem + L::kKV + L::kSegTile);
+            const uint32_t tS = tmem + 128 * t, tO = tmem + 256 + 128 * t;
+            bool ok = true;
+            uint32_t g = 0;                    // groups so far
+            uint32_t nq = 0, ns = 0, np = 0;   // this tile's items, scores and products so far
+            auto wait = [&](uint64_t* bar, uint32_t phase) { ok = ok && await(bar, phase, abort_flag, a.status); };
+            // The products that group g is for: O += P V of step g - 2 (if the tile has that step; `fresh`: its item's
+            // first) and S = Q K^T of step g (the same; begin, end: its item's first and last).  S goes where P of
+            // two steps before was, which the product before has read (MMAs run in order)
+            auto group = [&](bool output, bool fresh, bool scores, bool begin, bool end) {
+                const uint32_t place = SRC == kWide ? g & 3u : 2 * t + (g & 1u);
+                const uint32_t off = place * (L::kGroup >> 4);
+                const uint32_t kv_phase = (SRC == kWide ? g >> 2 : g >> 1) & 1u, p_phase = (np >> 1) & 1u;
+                uint64_t* const p_bar = p_full + 2 * t + (np & 1u);
+                const bool kv_there = mbar_try_wait(kv_full + place, kv_phase);
+                const bool p_there = !output || mbar_try_wait(p_bar, p_phase);
+                if (!kv_there) wait(kv_full + place, kv_phase);
+                if (scores && begin) wait(q_full + t, nq);
+                if (output) {
+                    const uint32_t buf = np & 1u;
+                    if (!p_there) wait(p_bar, p_phase);
+                    if (!ok) return;
                     tc_fence_after();
 #pragma unroll
-                    for (int k = 0; k < kTileKeys / 16; ++k)
-                        mma_ts(tO, tS + 8 * k, smem_desc_mn(v0 + k * 2048), id_o, (i - 1) | k);
-                    umma_commit(v_empty);
+                    for (int j = 0; j < kSeg / 16; ++j)
+                        mma_ts(tO, tS + 64 * buf + 8 * j, v0 + off + j * (2048 >> 4), id_o, j > 0 || !fresh);
+                    umma_commit(pv_done + t);
+                    ++np;
                 }
-                if (i < steps) {
-                    // S = Q K^T: it takes the place of P, which the product before has read (MMAs run in order)
-                    ok = mbar_wait(k_full, (uint32_t)i & 1u, abort_flag, a.status, kWaitNs);
-                    if (!ok) break;
+                if (scores) {
+                    if (!ok) return;
+                    const uint32_t buf = ns & 1u;
                     tc_fence_after();
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k)
-                        mma_ss(tS, smem_desc(q0 + (k / 4) * 16384 + (k % 4) * 32),
-                               smem_desc(k0 + (k / 4) * 16384 + (k % 4) * 32), id_s, k);
-                    umma_commit(k_empty);
-                    umma_commit(s_full);
+                    for (int j = 0; j < D / 16; ++j)
+                        mma_ss(tS + 64 * buf, q0 + (((j / 4) * 16384 + (j % 4) * 32) >> 4),
+                               k0 + off + (((j / 4) * L::kSegHalf + (j % 4) * 32) >> 4), id_s, j);
+                    umma_commit(s_full + 2 * t + buf);
+                    ++ns;
+                    if (end) {
+                        umma_commit(q_empty + t);
+                        ++nq;
+                    }
+                }
+                if (ok) umma_commit(kv_empty + place);
+                ++g;
+            };
+            // steps two and one before: does the tile have them, and are they their items' first?
+            bool has2 = false, has1 = false, first2 = false, first1 = false;
+            for (uint32_t item = blockIdx.x; ok && item < a.items; item += gridDim.x) {
+                const Item it = item_of<SRC>(a, item);
+                const bool has = t == 0 || it.both;
+                if (SRC == kBlocks && !has) continue;  // (there are no loads for it)
+                for (int i = 0; ok && i < it.steps; ++i) {
+                    group(has2, first2, has, i == 0, i + 1 == it.steps);
+                    has2 = has1;
+                    first2 = first1;
+                    has1 = has;
+                    first1 = i == 0;
                 }
             }
-            // on every way out: no MMA of this thread stays in flight
-            umma_commit(o_full);
+            if (ok && g > 0) {
+                group(has2, first2, false, false, false);
+                if (ok) group(has1, first1, false, false, false);
+            }
             if (!ok) {
+                // no MMA of this thread stays in flight
+                umma_commit(drain + t);
                 volatile int no_abort = 0;
-                mbar_wait(o_full, 0, &no_abort, nullptr, 100ull * 1000 * 1000);
+                mbar_wait(drain + t, 0, &no_abort, nullptr, 100ull * 1000 * 1000);
             }
         }
         __syncwarp();
-    } else if (warp > 4) {
-        if constexpr (SRC == kCodes) {
-            // ---------------- codes -> bf16 tiles
-            constexpr int kLanes = D / 16;          // threads along a token's channels, 16 codes each
-            constexpr int kRows = 128 / kLanes;     // tokens per pass
-            constexpr int kPasses = kTileKeys / kRows;
-            const int t = threadIdx.x - 160;
-            const int col = t % kLanes, row = t / kLanes;
-            const int8_t* src[2];
-#pragma unroll
-            for (int w = 0; w < 2; ++w) src[w] = a.codes[w] + (int64_t)h * a.cap * D + col * 16;
-            uint4 held[2][kPasses];
-            auto fetch = [&](int w, int i) {
-                const int64_t tok = (step0 + i) * kTileKeys + row;
-#pragma unroll
-                for (int p = 0; p < kPasses; ++p) {
-                    held[w][p] = make_uint4(0, 0, 0, 0);
-                    if (tok + p * kRows < a.keys)
-                        held[w][p] = __ldg(reinterpret_cast<const uint4*>(src[w] + (tok + p * kRows) * D));
-                }
-            };
-            auto store = [&](int w, uint8_t* tile) {
-                // 16 codes become two 16-byte pieces of the row's 128-byte half; the lanes of the upper half
-                // store them in the other order, so that eight lanes meet eight bank groups
-                uint8_t* half = tile + (col / 4) * 16384;
-                const int first = (col >> 2) & 1;
-#pragma unroll
-                for (int p = 0; p < kPasses; ++p) {
-                    const int r = row + p * kRows;
-                    const uint4 x = held[w][p];
-                    const uint4 lo = make_uint4(codes_to_bf16x2(x.x, 0x4140), codes_to_bf16x2(x.x, 0x4342),
-                                                codes_to_bf16x2(x.y, 0x4140), codes_to_bf16x2(x.y, 0x4342));
-                    const uint4 hi = make_uint4(codes_to_bf16x2(x.z, 0x4140), codes_to_bf16x2(x.z, 0x4342),
-                                                codes_to_bf16x2(x.w, 0x4140), codes_to_bf16x2(x.w, 0x4342));
-                    const int c0 = (col % 4) * 2 + first;
-                    *reinterpret_cast<uint4*>(half + r * 128 + ((c0 ^ (r & 7)) << 4)) = first ? hi : lo;
-                    *reinterpret_cast<uint4*>(half + r * 128 + (((c0 ^ 1) ^ (r & 7)) << 4)) = first ? lo : hi;
-                }
-            };
-            if (steps > 0) {
-                fetch(0, 0);
-                fetch(1, 0);
-            }
-            for (int i = 0; i < steps; ++i) {
-                const uint32_t ph = ((uint32_t)i & 1u) ^ 1u;
-                if (!mbar_wait(k_empty, ph, abort_flag, a.status, kWaitNs)) break;
-                store(0, sK);
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(k_full);
-                if (i + 1 < steps) fetch(0, i + 1);
-                if (!mbar_wait(v_empty, ph, abort_flag, a.status, kWaitNs)) break;
-                store(1, sV);
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(v_full);
-                if (i + 1 < steps) fetch(1, i + 1);
-            }
-        } else if (lane == 0) {
-            // ---------------- TMA loads; what is not there (a gap in the list, keys behind the last) lies
-            // outside the tensor and arrives as zeros
+    } else if (warp == 10) {
+        // ---------------- TMA loads, in the order in which the MMAs free their places.  What is not there (a gap
+        // in the list, keys behind the last) lies outside the tensor and arrives as zeros
+        if (lane == 0) {
             bool ok = true;
-            int k_armed = 0, v_armed = 0;
-            for (int i = 0; ok && i < steps; ++i) {
-                const uint32_t ph = ((uint32_t)i & 1u) ^ 1u;
-                int at[2];
+            uint32_t armed[4] = {0, 0, 0, 0}, nq[2] = {0, 0};  // loads so far into each place
+            auto load_q = [&](int t, const Where& w) {
+                ok = ok && await(q_empty + t, nq[t] + 1, abort_flag, a.status);  // (the first passes at once)
+                if (!ok) return;
+                mbar_expect_tx(q_full + t, L::kTile);
+                ++nq[t];
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const int64_t index = 2 * (step0 + i) + s;
-                    at[s] = (int)segment<SRC>(a, list, index, segs).at;
-                    if (SRC == kBlocks && index < segs) {
-                        const int64_t b = __ldg(list + index);
-                        if (b < -1 || b * kSeg >= a.keys) report(a.status, H3B_STATUS_BAD_INDEX);
+                for (int x = 0; x < L::kHalves; ++x)
+                    tma_load_3d(smem + L::kQ + t * L::kTile + x * 16384, &tmQ, q_full + t, x * 64, a.h0 + w.h, w.qt * kQRows);
+            };
+            struct Keys {
+                int h, at;  // head and first key, at < 0: none
+            };
+            auto load = [&](int place, const Keys& k, const Keys& v) {
+                ok = ok && await(kv_empty + place, armed[place] + 1, abort_flag, a.status);
+                if (!ok) return;
+                uint8_t* dst = smem + L::kKV + place * L::kGroup;
+                mbar_expect_tx(kv_full + place, (k.at >= 0 ? L::kSegTile : 0) + (v.at >= 0 ? L::kSegTile : 0));
+                ++armed[place];
+#pragma unroll
+                for (int x = 0; x < L::kHalves; ++x) {
+                    if (k.at >= 0) tma_load_3d(dst + x * L::kSegHalf, &tmK, kv_full + place, x * 64, k.h, k.at);
+                    if (v.at >= 0) tma_load_3d(dst + L::kSegTile + x * L::kSegHalf, &tmV, kv_full + place, x * 64, v.h, v.at);
+                }
+            };
+            const Keys none{0, -1};
+            Keys a1 = none, a2 = none, b1 = none, b2 = none;  // of the steps one and two before, tile 0's (or both's), 1's
+            uint32_t g0 = 0, g1 = 0;
+            auto place0 = [&] { return SRC == kWide ? (int)(g0 & 3u) : (int)(g0 & 1u); };
+            for (uint32_t item = blockIdx.x; ok && item < a.items; item += gridDim.x) {
+                const Item it = item_of<SRC>(a, item);
+                const Where w0 = where<SRC>(a, it.pair, 0), w1 = where<SRC>(a, it.pair, 1);
+                const int32_t *list0 = list_of<SRC>(a, w0), *list1 = list_of<SRC>(a, w1);
+                const bool own1 = SRC == kBlocks && it.both;
+                for (int i = 0; ok && i < it.steps; ++i) {
+                    // (looked up before the waits)
+                    const Seg s0 = segment<SRC>(a, list0, it.step0 + i);
+                    const Seg s1 = own1 ? segment<SRC>(a, list1, it.step0 + i) : Seg{0, 0};
+                    if (s0.n < 0 || s1.n < 0) report(a.status, H3B_STATUS_BAD_INDEX);
+                    if (i == 0) load_q(0, w0);
+                    const Keys k0{SRC == kWide ? w0.h : a.h0 + w0.h, s0.at}, k1{a.h0 + w1.h, s1.at};
+                    load(place0(), k0, a2);
+                    a2 = a1;
+                    a1 = k0;
+                    ++g0;
+                    if (i == 0 && it.both) load_q(1, w1);
+                    if (own1) {
+                        load(2 + (int)(g1 & 1u), k1, b2);
+                        b2 = b1;
+                        b1 = k1;
+                        ++g1;
                     }
                 }
-#pragma unroll
-                for (int w = 0; w < 2 && ok; ++w) {
-                    uint64_t* full = w ? v_full : k_full;
-                    if (!mbar_wait(w ? v_empty : k_empty, ph, abort_flag, a.status, kWaitNs)) {
-                        ok = false;
-                        break;
-                    }
-                    mbar_expect_tx(full, L::kTile);
-#pragma unroll
-                    for (int s = 0; s < 2; ++s)
-#pragma unroll
-                        for (int c = 0; c < L::kHalves; ++c)
-                            tma_load_3d((w ? sV : sK) + c * 16384 + s * 8192, w ? &tmV : &tmK, full, c * 64,
-                                        SRC == kBlocks ? h : hl, at[s]);
-                    ++(w ? v_armed : k_armed);
+            }
+            // the values of the last two steps
+            for (int j = 0; j < 2 && ok; ++j) {
+                load(place0(), none, j ? a1 : a2);
+                ++g0;
+                if (SRC == kBlocks && g1 > 0) {
+                    load(2 + (int)(g1 & 1u), none, j ? b1 : b2);
+                    ++g1;
                 }
             }
             if (!ok) {
                 // let the loads in flight land before the CTA exits
                 volatile int no_abort = 0;
-                if (k_armed) mbar_wait(k_full, (uint32_t)(k_armed - 1) & 1u, &no_abort, nullptr, 100ull * 1000 * 1000);
-                if (v_armed) mbar_wait(v_full, (uint32_t)(v_armed - 1) & 1u, &no_abort, nullptr, 100ull * 1000 * 1000);
+                for (int j = 0; j < 4; ++j)
+                    if (armed[j]) mbar_wait(kv_full + j, (armed[j] - 1u) & 1u, &no_abort, nullptr, 100ull * 1000 * 1000);
+                for (int t = 0; t < 2; ++t)
+                    if (nq[t]) mbar_wait(q_full + t, (nq[t] - 1u) & 1u, &no_abort, nullptr, 100ull * 1000 * 1000);
             }
         }
         __syncwarp();
     } else {
-        // ---------------- softmax, one query row a thread
-        const uint32_t at = (uint32_t)(warp * 32) << 16;
-        const int64_t row = qt * kQRows + threadIdx.x;
+        // ---------------- softmax and output of tile t, one query row a thread
+        const int t = warp >> 2, trow = threadIdx.x & 127;
+        const uint32_t at = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tS = tmem + at + 128 * t, tO = tmem + at + 256 + 128 * t;
         const float scale2 = fabsf(a.scale) * kLog2e;
-        Row st{-INFINITY, 0.0f};
+        // this tile's steps and outputs so far, and the uses of the output's place by both tiles
+        uint32_t step = 0, outs = 0, turn = 0;
         bool ok = true;
-        for (int i = 0; i < steps; ++i) {
-            int n[2];
-            float sk[2], sv[2];
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const Seg g = segment<SRC>(a, list, 2 * (step0 + i) + s, segs);
-                n[s] = g.n;
-                sk[s] = scale2;
-                sv[s] = 1.0f;
-                if (SRC != kBlocks && g.n > 0) {
-                    sk[s] = scale2 * __ldg(a.scales[0] + (int64_t)h * (a.cap / kSeg) + g.at / kSeg);
-                    sv[s] = __ldg(a.scales[1] + (int64_t)h * (a.cap / kSeg) + g.at / kSeg);
+        auto wait = [&](uint64_t* bar, uint32_t phase) {
+            return __all_sync(0xFFFFFFFFu, await(bar, phase, abort_flag, a.status)) != 0;
+        };
+        for (uint32_t item = blockIdx.x; ok && item < a.items; item += gridDim.x) {
+            const Item it = item_of<SRC>(a, item);
+            const Where u = where<SRC>(a, it.pair, t);
+            const int32_t* list = list_of<SRC>(a, u);
+            // (uses of the place alternate: by the time of a tile's next one its former one is over, since all its warps
+            // have taken part in a step after it)
+            const uint32_t mine = turn + t;
+            turn += it.both ? 2 : 1;
+            if (t == 1 && !it.both) continue;
+            Row st{-INFINITY, 0.0f};
+            for (int i = 0; ok && i < it.steps; ++i, ++step) {
+                const Seg g = segment<SRC>(a, list, it.step0 + i);
+                float sk = scale2, sv = 1.0f;
+                if (SRC == kWide) {
+                    const int64_t b = (int64_t)(a.h0 + u.h) * (a.cap / kSeg) + g.at / kSeg;
+                    sk = scale2 * __ldg(a.scales[0] + b);
+                    sv = __ldg(a.scales[1] + b);
                 }
+                const int buf = 2 * t + (int)(step & 1u);
+                if (!(ok = wait(s_full + buf, step >> 1))) break;
+                tc_fence_after();
+                const uint32_t tX = tS + 64 * (step & 1u);
+                auto product_done = [&] { ok = wait(pv_done + t, step - 1); };
+                if (g.n == kSeg)
+                    softmax_step<D, SRC, false>(st, tX, tO, i == 0, g.n, sk, sv, product_done);
+                else
+                    softmax_step<D, SRC, true>(st, tX, tO, i == 0, max(g.n, 0), sk, sv, product_done);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + buf);
             }
-            if (!(ok = mbar_wait(s_full, (uint32_t)i & 1u, abort_flag, a.status, kWaitNs))) break;
+            // one after the other: a wait tells a phase from the one before it only, and the last S came when all but
+            // the last two products were done
+            if (ok && step > 1) ok = wait(pv_done + t, step - 2);
+            if (!ok || !(ok = wait(pv_done + t, step - 1))) break;
             tc_fence_after();
-            if (n[0] + n[1] == kTileKeys)
-                softmax_step<D, SRC, false>(st, tS + at, tO + at, i > 0, n, sk, sv);
-            else
-                softmax_step<D, SRC, true>(st, tS + at, tO + at, i > 0, n, sk, sv);
-            tmem_st_wait();
+            const int64_t row = (int64_t)u.qt * kQRows + trow;
+            const bool split = a.parts > 1;
+            const float inv = st.l == 0.0f ? 0.0f : 1.0f / st.l;
+            const int64_t slot = ((int64_t)it.part * a.heads + u.h) * a.Sq + row;
+            if (split && row < a.Sq) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(st.m, st.l);
+            // the output's place is free when the store before has read it
+            if (!split && mine > 0 && !(ok = wait(out_free, mine - 1))) break;
+            // O: as it is to the join if this is a part of the keys, else through shared memory into whole rows of o
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t r[32];
+                tmem_ld32_async(tO + c * 32, r);
+                tmem_ready(r);
+                if (split) {
+                    if (row < a.Sq) {
+                        uint4* dst = reinterpret_cast<uint4*>(a.part_o + slot * D + c * 32);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) dst[e] = make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
+                    }
+                } else {
+                    uint8_t* half = smem + L::kO + (c / 2) * 16384 + trow * 128;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t o[4];
+#pragma unroll
+                        for (int f = 0; f < 4; ++f)
+                            o[f] = pack_bf16x2(__uint_as_float(r[8 * e + 2 * f]) * inv,
+                                               __uint_as_float(r[8 * e + 2 * f + 1]) * inv);
+                        *reinterpret_cast<uint4*>(half + ((((c & 1) * 4 + e) ^ (trow & 7)) << 4)) =
+                            make_uint4(o[0], o[1], o[2], o[3]);
+                    }
+                }
+            }
             tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full);
-        }
-        const float m = st.m, l = st.l;
-        if (ok && steps > 0) ok = mbar_wait(o_full, 0, abort_flag, a.status, kWaitNs);
-        tc_fence_after();
-        if (ok && gridDim.y > 1) {
-            // a part of the keys: O, its reference maximum and sum go to the join
-            const int64_t part = (int64_t)blockIdx.y * gridDim.x / a.nq * a.Sq + (int64_t)hl * a.Sq + row;
-            if (row < a.Sq) {
-                a.part_ml[2 * part] = m;
-                a.part_ml[2 * part + 1] = l;
-            }
+            if (!split) {
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(out_full + t);
+                if ((warp & 3) == 0) {
+                    if (!(ok = wait(out_full + t, outs))) break;
+                    if (lane == 0) {
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t r[32];
-                if (steps > 0) {
-                    tmem_ld32_async(tO + at + c * 32, r);
-                    tmem_ready(r);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) r[e] = 0;
-                }
-                if (row < a.Sq) {
-                    uint4* dst = reinterpret_cast<uint4*>(a.part_o + part * D + c * 32);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) dst[e] = make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
+                        for (int x = 0; x < L::kHalves; ++x)
+                            tma_store_3d(&tmO, smem + L::kO + x * 16384, x * 64, a.h0 + u.h, (int)(u.qt * kQRows));
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                        mbar_arrive(out_free);
+                    }
+                    __syncwarp();
                 }
             }
-        } else if (ok) {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            // through Q's place in shared memory (every MMA is done) into whole rows of o
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t r[32];
-                if (steps > 0) {
-                    tmem_ld32_async(tO + at + c * 32, r);
-                    tmem_ready(r);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) r[e] = 0;
-                }
-                uint8_t* half = sQ + (c / 2) * 16384 + threadIdx.x * 128;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    uint32_t o[4];
-#pragma unroll
-                    for (int f = 0; f < 4; ++f)
-                        o[f] = pack_bf16x2(__uint_as_float(r[8 * e + 2 * f]) * inv, __uint_as_float(r[8 * e + 2 * f + 1]) * inv);
-                    *reinterpret_cast<uint4*>(half + ((((c & 1) * 4 + e) ^ (threadIdx.x & 7)) << 4)) =
-                        make_uint4(o[0], o[1], o[2], o[3]);
-                }
-            }
-            fence_async_smem();
+            ++outs;
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (gridDim.y == 1 && !*abort_flag && threadIdx.x == 0) {
-#pragma unroll
-            for (int c = 0; c < L::kHalves; ++c) tma_store_3d(&tmO, sQ + c * 16384, c * 64, h, (int)(qt * kQRows));
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        }
+        // the stores have to be done before the CTA's memory goes
+        if (lane == 0 && (warp & 3) == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         __syncwarp();
     }
 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 4)
+    if (warp == 8)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
@@ -630,6 +735,14 @@ __global__ void __launch_bounds__(128) join_kernel(Args a, int heads, int parts)
     uint16_t* dst = a.o + row * a.o_ld + h * a.o_hs + lane * (D / 32);
 #pragma unroll
     for (int e = 0; e < D / 32; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(o[e] * inv, o[e + 1] * inv);
+}
+
+// o = 0 where there is no key at all, 8 channels a thread.
+__global__ void __launch_bounds__(256) zero_kernel(Args a, int per_head, int64_t pieces) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= pieces) return;
+    const int64_t row = i / per_head;
+    *reinterpret_cast<uint4*>(a.o + row / a.H * a.o_ld + row % a.H * a.o_hs + i % per_head * 8) = make_uint4(0, 0, 0, 0);
 }
 
 // Codes of some heads (each `per` pieces of 16 from `stride` pieces apart) -> bf16, K or V by blockIdx.y.
@@ -682,70 +795,67 @@ static int sm_count() {
     return cached;
 }
 
-// Parts that the keys of every row tile are split into.  All CTAs take about as
-// long, so the time is the number of rounds of two CTAs an SM times a part's
-// steps plus what a CTA spends besides (about two steps); a join costs about
-// two more.
-static int64_t parts_of(int64_t tiles, int64_t steps) {
-    const int64_t room = 2 * sm_count();
+// Parts that the keys of every row tile are split into.  All pairs of tiles take
+// about as long, so the time is the number of rounds of a pair an SM times a
+// part's steps plus what a pair spends besides (about four steps); a join costs
+// about four more.
+static int64_t parts_of(bool cache, int64_t nq, int64_t heads, int64_t steps) {
     int64_t best = 1, best_cost = 0;
-    for (int64_t n = 1; n <= 64 && (n == 1 || n * 2 <= steps); ++n) {
-        const int64_t cost = cdiv(tiles * n, room) * (cdiv(steps, n) + 2) + (n > 1 ? 2 : 0);
+    for (int64_t n = 1; n <= 64 && (n == 1 || n <= steps); ++n) {
+        const int64_t pairs = (cache ? cdiv(nq, 2) * heads : cdiv(nq * heads, 2)) * n;
+        const int64_t cost = cdiv(pairs, sm_count()) * (cdiv(steps, n) + 4) + (n > 1 ? 4 : 0);
         if (n == 1 || cost < best_cost) best = n, best_cost = cost;
     }
     return best;
 }
 
 struct Plan {
-    bool wide;          // the cache's codes are widened beforehand
-    int64_t heads;      // heads a launch (and of the widened copy)
-    int64_t parts;      // of the keys
+    int64_t heads;           // heads a launch (and of the widened copy)
+    int64_t parts;           // of the keys
     int64_t join_at, bytes;  // in the workspace
 };
 
-// From this many row tiles on a head's codes are widened once instead of by every CTA.
-constexpr int64_t kWideTiles = 4;
 constexpr int64_t kWideBytes = 256ll << 20;  // of widened heads at a time (one head at least)
 
 static Plan plan(bool cache, int64_t Sq, int64_t H, int64_t D, int64_t segs) {
-    Plan p{};
+    Plan p{H, 1, 0, 0};
+    if (segs == 0) return p;
     const int64_t nq = cdiv(Sq, kQRows);
-    p.wide = cache && nq >= kWideTiles && segs > 0;
-    const int64_t head = 2 * segs * kSeg * D * 2;
-    p.heads = H;
-    if (p.wide && H * head > kWideBytes) p.heads = kWideBytes / head > 0 ? kWideBytes / head : 1;
-    p.parts = parts_of(nq * p.heads, cdiv(segs, 2));
-    p.join_at = p.wide ? p.heads * head : 0;
+    const int64_t head = cache ? 2 * segs * kSeg * D * 2 : 0;
+    if (H * head > kWideBytes) p.heads = kWideBytes / head > 0 ? kWideBytes / head : 1;
+    p.parts = parts_of(cache, nq, p.heads, segs);
+    p.join_at = p.heads * head;
     p.bytes = p.join_at + (p.parts > 1 ? p.parts * p.heads * Sq * (D + 2) * 4 : 0);
     return p;
 }
 
 template <int D, Source SRC>
-static int launch_tiles(Args a, int64_t heads, int64_t parts, const uint16_t* const (&kv)[2], const int64_t (&ld)[2],
-                        const int64_t (&hs)[2], cudaStream_t s) {
-    CUtensorMap q{}, k{}, v{}, o{};
+static int launch_pairs(Args a, const uint16_t* const (&kv)[2], const int64_t (&ld)[2], const int64_t (&hs)[2],
+                        cudaStream_t s) {
+    CUtensorMap q, k, v, o;
     if (int rc = make_map(&q, a.q, a.Sq, a.H, D, a.q_ld, a.q_hs, kQRows)) return rc;
     if (int rc = make_map(&o, a.o, a.Sq, a.H, D, a.o_ld, a.o_hs, kQRows)) return rc;
-    if (SRC != kCodes && a.keys > 0) {
-        const int n = SRC == kBlocks ? a.H : (int)heads;
-        if (int rc = make_map(&k, kv[0], a.keys, n, D, ld[0], hs[0], kSeg)) return rc;
-        if (int rc = make_map(&v, kv[1], a.keys, n, D, ld[1], hs[1], kSeg)) return rc;
-    }
-    H3B_CUDA_TRY(cudaFuncSetAttribute(tile_kernel<D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes));
-    const dim3 grid((unsigned)(a.nq * heads), (unsigned)parts);
-    tile_kernel<D, SRC><<<grid, tile_threads<SRC>(), Smem<D>::kBytes, s>>>(q, k, v, o, a);
-    if (parts > 1) join_kernel<D><<<(unsigned)cdiv(a.Sq * heads, 4), 128, 0, s>>>(a, (int)heads, (int)parts);
+    const int n = SRC == kBlocks ? a.H : a.heads;
+    if (int rc = make_map(&k, kv[0], a.keys, n, D, ld[0], hs[0], kSeg)) return rc;
+    if (int rc = make_map(&v, kv[1], a.keys, n, D, ld[1], hs[1], kSeg)) return rc;
+    const int64_t items = (SRC == kWide ? cdiv(a.nq, 2) * a.heads : cdiv(a.nq * a.heads, 2)) * a.parts;
+    a.items = (uint32_t)items;
+    H3B_CUDA_TRY(cudaFuncSetAttribute(pair_kernel<D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes));
+    const int64_t grid = items < sm_count() ? items : sm_count();
+    pair_kernel<D, SRC><<<(unsigned)grid, kPairThreads, Smem<D>::kBytes, s>>>(q, k, v, o, a);
+    if (a.parts > 1) join_kernel<D><<<(unsigned)cdiv(a.Sq * a.heads, 4), 128, 0, s>>>(a, a.heads, a.parts);
     H3B_CUDA_TRY(cudaGetLastError());
     return H3B_OK;
 }
 
 template <int D>
-static int launch_all(Args& a, bool cache, const Plan& p, int64_t segs, char* ws, cudaStream_t s) {
+static int launch_all(Args& a, bool cache, const Plan& p, char* ws, cudaStream_t s) {
     a.part_o = reinterpret_cast<float*>(ws + p.join_at);
     a.part_ml = a.part_o + (p.parts > 1 ? p.parts * p.heads * a.Sq * D : 0);
-    if (!cache) return launch_tiles<D, kBlocks>(a, a.H, p.parts, a.kv, a.kv_ld, a.kv_hs, s);
-    if (!p.wide) return launch_tiles<D, kCodes>(a, a.H, p.parts, a.kv, a.kv_ld, a.kv_hs, s);
-    const int64_t rows = segs * kSeg;
+    a.parts = (int)p.parts;
+    a.heads = a.H;
+    if (!cache) return launch_pairs<D, kBlocks>(a, a.kv, a.kv_ld, a.kv_hs, s);
+    const int64_t rows = a.segs * kSeg;
     uint16_t* const k = reinterpret_cast<uint16_t*>(ws);
     for (int64_t h = 0; h < a.H; h += p.heads) {
         const int64_t n = a.H - h < p.heads ? a.H - h : p.heads;
@@ -754,9 +864,10 @@ static int launch_all(Args& a, bool cache, const Plan& p, int64_t segs, char* ws
         widen_kernel<<<dim3((unsigned)cdiv(pieces, 4 * 256), 2), 256, 0, s>>>(
             a.codes[0] + h * a.cap * D, a.codes[1] + h * a.cap * D, a.cap * D / 16, rows * D / 16, pieces, k, v);
         a.h0 = (int)h;
+        a.heads = (int)n;
         const int64_t ld[2] = {D, D}, hs[2] = {rows * D, rows * D};
         const uint16_t* const kv[2] = {k, v};
-        if (int rc = launch_tiles<D, kWide>(a, n, p.parts, kv, ld, hs, s)) return rc;
+        if (int rc = launch_pairs<D, kWide>(a, kv, ld, hs, s)) return rc;
     }
     return H3B_OK;
 }
@@ -772,16 +883,24 @@ static int launch(const char* who, bool cache, Args& a, int64_t D, int64_t segs,
     H3B_REQUIRE(a.q_ld > 0 && a.q_hs > 0 && a.o_ld > 0 && a.o_hs > 0 && a.q_ld % 8 == 0 && a.q_hs % 8 == 0 &&
                     a.o_ld % 8 == 0 && a.o_hs % 8 == 0,
                 "%s: strides must be positive multiples of 8 elements", who);
+    if (a.keys == 0) segs = 0;
+    a.segs = segs;
     a.nq = cdiv(a.Sq, kQRows);
-    H3B_REQUIRE(a.nq * a.H < (1ll << 31) && a.Sq * a.H < (1ll << 33), "%s: too many row tiles", who);
     const Plan p = plan(cache, a.Sq, a.H, D, segs);
+    H3B_REQUIRE(a.nq * a.H * p.parts < (1ll << 30) && a.Sq * a.H < (1ll << 33), "%s: too many row tiles", who);
     H3B_REQUIRE(p.bytes == 0 || (ws && aligned(ws, 256) && ws_bytes >= p.bytes),
                 "%s: workspace of %lld bytes (256-byte aligned), %lld needed", who, (long long)ws_bytes, (long long)p.bytes);
     DeviceStatus ds;
     if (int rc = device_status(&ds)) return rc;
     a.status = ds.word;
-    return D == 128 ? launch_all<128>(a, cache, p, segs, static_cast<char*>(ws), s)
-                    : launch_all<64>(a, cache, p, segs, static_cast<char*>(ws), s);
+    if (segs == 0) {
+        const int64_t pieces = a.Sq * a.H * D / 8;
+        zero_kernel<<<(unsigned)cdiv(pieces, 256), 256, 0, s>>>(a, (int)(D / 8), pieces);
+        H3B_CUDA_TRY(cudaGetLastError());
+        return H3B_OK;
+    }
+    return D == 128 ? launch_all<128>(a, cache, p, static_cast<char*>(ws), s)
+                    : launch_all<64>(a, cache, p, static_cast<char*>(ws), s);
 }
 
 }  // namespace attn

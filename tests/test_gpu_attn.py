@@ -509,3 +509,27 @@ def test_model_with_text_cache_and_sparse_attention():
     y = dense.forward(x.clone(), ridx, None, caches)
     assert torch.isfinite(y).all() and not same(y, plain)
     assert h3b.status() == 0
+
+
+@pytest.mark.parametrize("rows,tokens,H", [(300, 70, 40), (900, 200, 40), (16000 // 8 - 40, 512, 40), (130, 1500, 150)])
+def test_cached_attention_with_an_odd_number_of_tiles_over_many_items(rows, tokens, H):
+    """More pairs of row tiles than SMs, and a head's last pair with one tile only: CTAs that go from item to item."""
+    c = filled(H, -(-tokens // 64) * 64, 128, tokens, seed=rows)
+    q = randn(rows, H, 128, seed=tokens)
+    got = h3b.kv8_attention(q, c)
+    k, v = values(c)
+    for h in (0, 1, H // 2, H - 1):
+        o, a, m = softmax_rows(q[:, h], k[:, h], v[:, h], 128 ** -0.5)
+        near(got[:, h], o, a, m, tokens, 128)
+    assert same(got[:, ::7], h3b.kv8_attention(q, c)[:, ::7])
+    assert h3b.status() == 0
+
+
+@pytest.mark.parametrize("rows,H", [(129, 150), (640, 40), (385, 149)])
+def test_sparse_attention_over_many_items(rows, H):
+    q, k, v = randn(rows, H, 64, seed=1), randn(400, H, 64, seed=2), randn(400, H, 64, seed=3)
+    o, blocks = h3b.sparse_attention(q, k, v, 3, return_blocks=True)
+    heads = [0, H // 3, H - 1]
+    ref, a, m = sparse(q[:, heads], k[:, heads], v[:, heads], blocks[heads], 64 ** -0.5)
+    near(o[:, heads], ref, a, m, 192, 64)
+    assert h3b.status() == 0
