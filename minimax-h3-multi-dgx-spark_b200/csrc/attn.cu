@@ -50,7 +50,7 @@ struct Args {
 // time: the chain of a step took 3700 clocks, of which 1024 are products.)
 
 constexpr int kTmemCols = 512;     // S of tile t at 128 t (+ 64 for odd steps), O at 256 + 128 t
-constexpr int kPairThreads = 352;  // 2 x 4 softmax warps, an MMA warp for each tile, the TMA warp
+constexpr int kPairThreads = 384;  // 2 x 4 softmax warps, an MMA warp and a TMA warp for each tile
 constexpr uint64_t kWaitNs = 1000ull * 1000 * 1000;
 constexpr float kLog2e = 1.4426950408889634f;
 // A row's reference maximum moves when a score exceeds it by 2^8: until then p
@@ -109,16 +109,18 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
         : "memory");
 }
 
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
+// [tokens, heads, D] bf16 seen as (64 channels, tokens, halves of D, heads): a box
+// lands as whole 128-byte rows, the halves of D one behind the other.
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, uint64_t* bar, int token, int head) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %3, %5}], [%2];" ::"r"(
             smem_u32(dst)),
-        "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+        "l"(map), "r"(smem_u32(bar)), "r"(0), "r"(token), "r"(head)
         : "memory");
 }
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int c0, int c1, int c2) {
-    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
-                 "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2)
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, const void* src, int token, int head) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %2, %4}], [%1];" ::"l"(map),
+                 "r"(smem_u32(src)), "r"(0), "r"(token), "r"(head)
                  : "memory");
 }
 
@@ -517,81 +519,67 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             }
         }
         __syncwarp();
-    } else if (warp == 10) {
-        // ---------------- TMA loads, in the order in which the MMAs free their places.  What is not there (a gap
-        // in the list, keys behind the last) lies outside the tensor and arrives as zeros
+    } else if (warp == 10 || warp == 11) {
+        // ---------------- TMA loads of tile t (keys and values of kWide by the first warp alone), in the order in
+        // which the MMAs free their places.  What is not there (a gap in the list, keys behind the last) lies outside
+        // the tensor and arrives as zeros
         if (lane == 0) {
+            const int t = warp - 10;
+            const bool loads = SRC == kBlocks || t == 0;
             bool ok = true;
-            uint32_t armed[4] = {0, 0, 0, 0}, nq[2] = {0, 0};  // loads so far into each place
-            auto load_q = [&](int t, const Where& w) {
-                ok = ok && await(q_empty + t, nq[t] + 1, abort_flag, a.status);  // (the first passes at once)
-                if (!ok) return;
-                mbar_expect_tx(q_full + t, L::kTile);
-                ++nq[t];
-#pragma unroll
-                for (int x = 0; x < L::kHalves; ++x)
-                    tma_load_3d(smem + L::kQ + t * L::kTile + x * 16384, &tmQ, q_full + t, x * 64, a.h0 + w.h, w.qt * kQRows);
-            };
+            uint32_t armed[4] = {0, 0, 0, 0}, nq = 0, g = 0;  // loads so far into each place, items, groups
+            // a step's keys are loaded with the values of the step two before it; at < 0: none
             struct Keys {
-                int h, at;  // head and first key, at < 0: none
+                int h, at;
             };
-            auto load = [&](int place, const Keys& k, const Keys& v) {
-                ok = ok && await(kv_empty + place, armed[place] + 1, abort_flag, a.status);
+            auto load = [&](const Keys& k, const Keys& v) {
+                const int place = (int)(SRC == kWide ? g & 3u : 2 * t + (g & 1u));
+                uint32_t& n = armed[SRC == kWide ? g & 3u : g & 1u];
+                ok = ok && await(kv_empty + place, n + 1, abort_flag, a.status);  // (the first passes at once)
                 if (!ok) return;
                 uint8_t* dst = smem + L::kKV + place * L::kGroup;
                 mbar_expect_tx(kv_full + place, (k.at >= 0 ? L::kSegTile : 0) + (v.at >= 0 ? L::kSegTile : 0));
-                ++armed[place];
-#pragma unroll
-                for (int x = 0; x < L::kHalves; ++x) {
-                    if (k.at >= 0) tma_load_3d(dst + x * L::kSegHalf, &tmK, kv_full + place, x * 64, k.h, k.at);
-                    if (v.at >= 0) tma_load_3d(dst + L::kSegTile + x * L::kSegHalf, &tmV, kv_full + place, x * 64, v.h, v.at);
-                }
+                ++n;
+                ++g;
+                if (k.at >= 0) tma_load(dst, &tmK, kv_full + place, k.at, k.h);
+                if (v.at >= 0) tma_load(dst + L::kSegTile, &tmV, kv_full + place, v.at, v.h);
             };
-            const Keys none{0, -1};
-            Keys a1 = none, a2 = none, b1 = none, b2 = none;  // of the steps one and two before, tile 0's (or both's), 1's
-            uint32_t g0 = 0, g1 = 0;
-            auto place0 = [&] { return SRC == kWide ? (int)(g0 & 3u) : (int)(g0 & 1u); };
+            Keys k1{0, -1}, k2{0, -1};  // of the steps one and two before
             for (uint32_t item = blockIdx.x; ok && item < a.items; item += gridDim.x) {
                 const Item it = item_of<SRC>(a, item);
-                const Where w0 = where<SRC>(a, it.pair, 0), w1 = where<SRC>(a, it.pair, 1);
-                const int32_t *list0 = list_of<SRC>(a, w0), *list1 = list_of<SRC>(a, w1);
-                const bool own1 = SRC == kBlocks && it.both;
-                for (int i = 0; ok && i < it.steps; ++i) {
-                    // (looked up before the waits)
-                    const Seg s0 = segment<SRC>(a, list0, it.step0 + i);
-                    const Seg s1 = own1 ? segment<SRC>(a, list1, it.step0 + i) : Seg{0, 0};
-                    if (s0.n < 0 || s1.n < 0) report(a.status, H3B_STATUS_BAD_INDEX);
-                    if (i == 0) load_q(0, w0);
-                    const Keys k0{SRC == kWide ? w0.h : a.h0 + w0.h, s0.at}, k1{a.h0 + w1.h, s1.at};
-                    load(place0(), k0, a2);
-                    a2 = a1;
-                    a1 = k0;
-                    ++g0;
-                    if (i == 0 && it.both) load_q(1, w1);
-                    if (own1) {
-                        load(2 + (int)(g1 & 1u), k1, b2);
-                        b2 = b1;
-                        b1 = k1;
-                        ++g1;
-                    }
+                if (t == 1 && !it.both) continue;
+                const Where w = where<SRC>(a, it.pair, t);
+                const int32_t* list = list_of<SRC>(a, w);
+                // (blocks are looked up a step ahead of their load)
+                Seg seg = loads ? segment<SRC>(a, list, it.step0) : Seg{0, 0};
+                ok = ok && await(q_empty + t, nq + 1, abort_flag, a.status);
+                if (!ok) break;
+                mbar_expect_tx(q_full + t, L::kTile);
+                ++nq;
+                tma_load(smem + L::kQ + t * L::kTile, &tmQ, q_full + t, w.qt * kQRows, a.h0 + w.h);
+                for (int i = 0; ok && loads && i < it.steps; ++i) {
+                    const Seg next = i + 1 < it.steps ? segment<SRC>(a, list, it.step0 + i + 1) : seg;
+                    if (seg.n < 0) report(a.status, H3B_STATUS_BAD_INDEX);
+                    const Keys k{SRC == kWide ? w.h : a.h0 + w.h, seg.at};
+                    load(k, k2);
+                    k2 = k1;
+                    k1 = k;
+                    seg = next;
                 }
             }
             // the values of the last two steps
-            for (int j = 0; j < 2 && ok; ++j) {
-                load(place0(), none, j ? a1 : a2);
-                ++g0;
-                if (SRC == kBlocks && g1 > 0) {
-                    load(2 + (int)(g1 & 1u), none, j ? b1 : b2);
-                    ++g1;
-                }
+            if (loads && g > 0) {
+                load(Keys{0, -1}, k2);
+                load(Keys{0, -1}, k1);
             }
             if (!ok) {
                 // let the loads in flight land before the CTA exits
                 volatile int no_abort = 0;
                 for (int j = 0; j < 4; ++j)
-                    if (armed[j]) mbar_wait(kv_full + j, (armed[j] - 1u) & 1u, &no_abort, nullptr, 100ull * 1000 * 1000);
-                for (int t = 0; t < 2; ++t)
-                    if (nq[t]) mbar_wait(q_full + t, (nq[t] - 1u) & 1u, &no_abort, nullptr, 100ull * 1000 * 1000);
+                    if (armed[j])
+                        mbar_wait(kv_full + (SRC == kWide ? j : 2 * t + j), (armed[j] - 1u) & 1u, &no_abort, nullptr,
+                                  100ull * 1000 * 1000);
+                if (nq) mbar_wait(q_full + t, (nq - 1u) & 1u, &no_abort, nullptr, 100ull * 1000 * 1000);
             }
         }
         __syncwarp();
@@ -617,23 +605,30 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             turn += it.both ? 2 : 1;
             if (t == 1 && !it.both) continue;
             Row st{-INFINITY, 0.0f};
-            for (int i = 0; ok && i < it.steps; ++i, ++step) {
+            struct Factors {
+                int n;
+                float sk, sv;
+            };
+            auto factors = [&](int i) {
                 const Seg g = segment<SRC>(a, list, it.step0 + i);
-                float sk = scale2, sv = 1.0f;
-                if (SRC == kWide) {
-                    const int64_t b = (int64_t)(a.h0 + u.h) * (a.cap / kSeg) + g.at / kSeg;
-                    sk = scale2 * __ldg(a.scales[0] + b);
-                    sv = __ldg(a.scales[1] + b);
-                }
+                if (SRC == kBlocks) return Factors{g.n, scale2, 1.0f};
+                const int64_t b = (int64_t)(a.h0 + u.h) * (a.cap / kSeg) + it.step0 + i;
+                return Factors{g.n, __ldg(a.scales[0] + b), __ldg(a.scales[1] + b)};
+            };
+            Factors ahead = factors(0);
+            for (int i = 0; ok && i < it.steps; ++i, ++step) {
+                const Factors f = ahead;
+                if (i + 1 < it.steps) ahead = factors(i + 1);
                 const int buf = 2 * t + (int)(step & 1u);
                 if (!(ok = wait(s_full + buf, step >> 1))) break;
                 tc_fence_after();
                 const uint32_t tX = tS + 64 * (step & 1u);
                 auto product_done = [&] { ok = wait(pv_done + t, step - 1); };
-                if (g.n == kSeg)
-                    softmax_step<D, SRC, false>(st, tX, tO, i == 0, g.n, sk, sv, product_done);
+                const float sk = SRC == kBlocks ? scale2 : scale2 * f.sk;
+                if (f.n == kSeg)
+                    softmax_step<D, SRC, false>(st, tX, tO, i == 0, f.n, sk, f.sv, product_done);
                 else
-                    softmax_step<D, SRC, true>(st, tX, tO, i == 0, max(g.n, 0), sk, sv, product_done);
+                    softmax_step<D, SRC, true>(st, tX, tO, i == 0, max(f.n, 0), sk, f.sv, product_done);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -685,9 +680,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 if ((warp & 3) == 0) {
                     if (!(ok = wait(out_full + t, outs))) break;
                     if (lane == 0) {
-#pragma unroll
-                        for (int x = 0; x < L::kHalves; ++x)
-                            tma_store_3d(&tmO, smem + L::kO + x * 16384, x * 64, a.h0 + u.h, (int)(u.qt * kQRows));
+                        tma_store(&tmO, smem + L::kO, u.qt * kQRows, a.h0 + u.h);
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                         asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                         mbar_arrive(out_free);
@@ -769,15 +762,15 @@ __global__ void __launch_bounds__(256) widen_kernel(const int8_t* __restrict__ k
     }
 }
 
-// [tokens, heads, D] bf16 as boxes of `rows` tokens x 64 channels of a head.
+// [tokens, heads, D] bf16 as boxes of `rows` tokens of a head (see tma_load).
 static int make_map(CUtensorMap* map, const void* p, int64_t n, int H, int64_t D, int64_t ld, int64_t hs, int rows) {
     PFN_encodeTiled enc = encode_fn();
     if (!enc) return set_error(H3B_ERR_CUDA, "cuTensorMapEncodeTiled unavailable (driver too old?)");
-    cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)n};
-    cuuint64_t strides[2] = {(cuuint64_t)hs * 2, (cuuint64_t)ld * 2};
-    cuuint32_t box[3] = {64, 1, (cuuint32_t)rows};
-    cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, estr,
+    cuuint64_t dims[4] = {64, (cuuint64_t)n, (cuuint64_t)(D / 64), (cuuint64_t)H};
+    cuuint64_t strides[3] = {(cuuint64_t)ld * 2, 128, (cuuint64_t)hs * 2};
+    cuuint32_t box[4] = {64, (cuuint32_t)rows, (cuuint32_t)(D / 64), 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(p), dims, strides, box, estr,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(H3B_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
