@@ -1,6 +1,8 @@
 // Attention over a key/value cache held in 8 bits, and over selected blocks of
 // bf16 keys:  o = softmax(scale * q k^T) v, one pass over the keys with the
 // running maximum and sum of the softmax.
+#include <type_traits>
+
 #include "ptx.cuh"
 
 namespace h3b {
@@ -202,15 +204,20 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     return d;
 }
 
-// Two int8 codes (bytes `sel` picks, zero-extended to 16 bits) -> bf16x2, exactly:
-// in [128, 256) a bf16 steps by 1, so 0x4300 | low 7 bits is 128 + them, and
-// 0x4300 | sign bit is 128, or 256 for a negative code.
-__device__ __forceinline__ uint32_t codes_to_bf16x2(uint32_t x, uint32_t sel) {
-    const uint32_t t = __byte_perm(x, 0, sel);
+// Two int8 codes (in bytes 0 and 2; what is in the others does not matter) ->
+// bf16x2, exactly: in [128, 256) a bf16 steps by 1, so 0x4300 | low 7 bits is 128
+// + them, and 0x4300 | sign bit is 128, or 256 for a negative code.
+__device__ __forceinline__ uint32_t widen2(uint32_t t) {
     const uint32_t a = (t & 0x007F007Fu) | 0x43004300u, b = (t & 0x00800080u) | 0x43004300u;
     const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
                                      *reinterpret_cast<const __nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&d);
+}
+// bytes 0 and 1 (sel 0x4140) or 2 and 3 (0x4342) of a word
+__device__ __forceinline__ uint32_t codes_to_bf16x2(uint32_t x, uint32_t sel) { return widen2(__byte_perm(x, 0, sel)); }
+// byte i of two words
+__device__ __forceinline__ uint32_t code_pair(uint32_t x, uint32_t y, int i) {
+    return widen2(__byte_perm(x, y, i | ((4 + i) << 8)));
 }
 
 // Where a tile's keys and values come from.
@@ -702,32 +709,265 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
-// Join of the parts of a split: o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.  One warp a row.
+// ---------------------------------------------------------------------------
+// Rows kernel: few query rows over the cache.  The codes are read once, straight
+// into registers, and widened there as operands of mma.sync m16n8k16: 16 query
+// rows a warp, 16 keys a turn.  Which channel (of the scores) or key and channel
+// (of the output) an operand's register stands for is ours to choose, as long as
+// both operands agree, so every thread loads 16 (or 8) consecutive codes:
+//   scores   thread (g, c) = (lane / 4, lane % 4) holds D / 4 channels of keys
+//            4 (g / 2) + g % 2 and two behind it
+//   output   D / 8 channels of keys 4 c .. 4 c + 3
+// The scores' accumulators then are the output product's P operand as they lie.
+// What bounds it is the cache's bytes: 16 rows take about 2 instructions a clock
+// and SM at the rate at which HBM delivers them.
+
+constexpr int kFewRows = 16;   // query rows a warp
+constexpr int kRowWarps = 4;   // of a CTA, each with its own segments
+// Up to this many rows the rows kernel reads the codes once per 16 rows (from L2
+// after the first); beyond, they are widened once for the pair kernel.
+constexpr int64_t kRowsMost = 64;
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 template <int D>
-__global__ void __launch_bounds__(128) join_kernel(Args a, int heads, int parts) {
-    const int lane = threadIdx.x & 31;
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int64_t step = a.Sq * heads;
-    if (id >= step) return;
+__global__ void __launch_bounds__(32 * kRowWarps, 2) rows_kernel(const __grid_constant__ Args a) {
+    constexpr int kC = D / 4;        // channels of a thread's keys (scores)
+    constexpr int kN = D / 8;        // channels of a thread (output), and n-tiles of 8 channels
+    constexpr int kKW = kC / 16;     // uint4 a key
+    using Piece = typename std::conditional<D == 128, uint4, uint2>::type;  // kN codes
+    __shared__ float so[kRowWarps][kFewRows][D];
+    __shared__ float sm[kRowWarps][kFewRows], sl[kRowWarps][kFewRows];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+    // row groups first: CTAs that run together share a head's codes in L2
+    const uint32_t groups = (uint32_t)((a.Sq + kFewRows - 1) / kFewRows);
+    const uint32_t rest = blockIdx.x / groups;
+    const int64_t row0 = (int64_t)(blockIdx.x - rest * groups) * kFewRows;
+    const int part = (int)(rest / (uint32_t)a.H), h = (int)(rest - part * (uint32_t)a.H);
+    const int rows = (int)min((int64_t)kFewRows, a.Sq - row0);
+
+    uint32_t q[kC / 4][4];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const uint16_t* src = a.q + (row0 + g + 8 * r) * a.q_ld + h * a.q_hs + c * kC;
+#pragma unroll
+        for (int j = 0; j < kC / 8; ++j) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (g + 8 * r < rows) x = *reinterpret_cast<const uint4*>(src + 8 * j);
+            q[2 * j][r] = x.x;
+            q[2 * j][r + 2] = x.y;
+            q[2 * j + 1][r] = x.z;
+            q[2 * j + 1][r + 2] = x.w;
+        }
+    }
+
+    float o[kN][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < kN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+
+    // this warp's segments: seg0, seg0 + kRowWarps, .. below seg1
+    const int64_t segs = a.segs, seg1 = segs * (part + 1) / a.parts;
+    const int64_t seg0 = segs * part / a.parts + warp;
+    const int8_t* kbase = a.codes[0] + ((int64_t)h * a.cap + 4 * (g >> 1) + (g & 1)) * D + c * kC;
+    const int8_t* vbase = a.codes[1] + ((int64_t)h * a.cap + 4 * c) * D + g * kN;
+    const float* ks = a.scales[0] + (int64_t)h * (a.cap / kSeg);
+    const float* vs = a.scales[1] + (int64_t)h * (a.cap / kSeg);
+    const float scale2 = a.scale * kLog2e;
+    uint4 kx[2][kKW];
+    Piece vx[4];
+    auto fetch = [&](int64_t seg, int turn) {
+        const int64_t at = (seg * kSeg + turn * 16) * D;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int w = 0; w < kKW; ++w)
+                kx[t][w] = __ldcs(reinterpret_cast<const uint4*>(kbase + at + t * 2 * D) + w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) vx[k] = __ldcs(reinterpret_cast<const Piece*>(vbase + at + k * D));
+    };
+    float sk = 0.0f, sv = 0.0f;
+    if (seg0 < seg1) {
+        fetch(seg0, 0);
+        sk = __ldg(ks + seg0);
+        sv = __ldg(vs + seg0);
+    }
+    for (int64_t seg = seg0; seg < seg1; seg += kRowWarps) {
+        const float fk = sk * scale2, fv = sv;
+        const int valid = (int)min((int64_t)kSeg, a.keys - seg * kSeg);
+        const bool more = seg + kRowWarps < seg1;
+        if (more) {
+            sk = __ldg(ks + seg + kRowWarps);
+            sv = __ldg(vs + seg + kRowWarps);
+        }
+#pragma unroll 1
+        for (int turn = 0; turn < kSeg / 16; ++turn) {
+            uint4 kc[2][kKW];
+            Piece vc[4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int w = 0; w < kKW; ++w) kc[t][w] = kx[t][w];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) vc[k] = vx[k];
+            if (turn + 1 < kSeg / 16) fetch(seg, turn + 1);
+            else if (more) fetch(seg + kRowWarps, 0);
+            // scores: two n-tiles, of keys 4 c, 4 c + 1 and of keys 4 c + 2, 4 c + 3 in this thread
+            float s[2][4] = {};
+#pragma unroll
+            for (int j = 0; j < kC / 4; ++j)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const uint4 x = kc[t][j / 4];
+                    const uint32_t w = j % 4 == 0 ? x.x : j % 4 == 1 ? x.y : j % 4 == 2 ? x.z : x.w;
+                    mma_16816(s[t], q[j], codes_to_bf16x2(w, 0x4140), codes_to_bf16x2(w, 0x4342));
+                }
+            const int left = valid - turn * 16 - 4 * c;  // of this thread's four keys
+            float x[2][4];                               // [row half][key]
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float y = s[k >> 1][2 * r + (k & 1)] * fk;
+                    x[r][k] = k < left ? y : -INFINITY;
+                }
+            float top[2];
+            bool moves = false;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                top[r] = fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]));
+                moves |= top[r] > m[r] + kSlack || (m[r] == -INFINITY && top[r] > m[r]);
+            }
+            if (__any_sync(0xFFFFFFFFu, moves)) {
+                float keep[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 1));
+                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 2));
+                    const float to = fmaxf(m[r], top[r]);
+                    keep[r] = to == m[r] ? 1.0f : ex2(m[r] - to);
+                    m[r] = to;
+                    l[r] *= keep[r];
+                }
+#pragma unroll
+                for (int j = 0; j < kN; ++j) {
+                    o[j][0] *= keep[0];
+                    o[j][1] *= keep[0];
+                    o[j][2] *= keep[1];
+                    o[j][3] *= keep[1];
+                }
+            }
+            uint32_t p[4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float ref = m[r] == -INFINITY ? 0.0f : m[r];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    x[r][k] = ex2(x[r][k] - ref);
+                    l[r] += x[r][k];
+                    x[r][k] *= fv;
+                }
+                // p is rounded to bf16 for the second product (its sum is not): a relative 2^-8 at most a key
+                p[r] = pack_bf16x2(x[r][0], x[r][1]);
+                p[r + 2] = pack_bf16x2(x[r][2], x[r][3]);
+            }
+            // output: n-tile j has channel kN g + j in this thread, whose keys are bytes of four different words
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = reinterpret_cast<const uint32_t*>(&vc[k])[j / 4];
+                mma_16816(o[j], p, code_pair(w[0], w[1], j % 4), code_pair(w[2], w[3], j % 4));
+            }
+        }
+    }
+    // the warps' parts meet in shared memory
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
+        if (c == 0) {
+            sm[warp][g + 8 * r] = m[r];
+            sl[warp][g + 8 * r] = l[r];
+        }
+        // accumulator columns 2 c, 2 c + 1 of n-tile j are its rows' channels kN (2 c) + j and kN (2 c + 1) + j
+        if (g + 8 * r < rows) {
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                so[warp][g + 8 * r][kN * 2 * c + j] = o[j][2 * r];
+                so[warp][g + 8 * r][kN * (2 * c + 1) + j] = o[j][2 * r + 1];
+            }
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * (D / 2); e += 32 * kRowWarps) {
+        const int r = e / (D / 2), ch = 2 * (e % (D / 2));
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm[w][r]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float total = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) {
+            const float f = ex2(sm[w][r] - ref);
+            total += f * sl[w][r];
+            x += f * so[w][r][ch];
+            y += f * so[w][r][ch + 1];
+        }
+        if (a.parts > 1) {
+            const int64_t slot = ((int64_t)part * a.H + h) * a.Sq + row0 + r;
+            *reinterpret_cast<float2*>(a.part_o + slot * D + ch) = make_float2(x, y);
+            if (ch == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(top, total);
+        } else {
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            *reinterpret_cast<uint32_t*>(a.o + (row0 + r) * a.o_ld + h * a.o_hs + ch) = pack_bf16x2(x * inv, y * inv);
+        }
+    }
+}
+
+// Join of the parts of a split: o = sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.
+// One CTA a row and head; its warps take the parts in turn.
+template <int D>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args a) {
+    constexpr int E = D / 32;
+    __shared__ float so[4][D], sl[4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t id = blockIdx.x, step = a.Sq * a.heads;
     const int h = a.h0 + (int)(id / a.Sq);
     const int64_t row = id % a.Sq;
     float m = -INFINITY;
-    for (int s = lane; s < parts; s += 32) m = fmaxf(m, a.part_ml[2 * (s * step + id)]);
+    for (int s = lane; s < a.parts; s += 32) m = fmaxf(m, a.part_ml[2 * (s * step + id)]);
 #pragma unroll
     for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
     const float ref = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, o[D / 32] = {};
-    for (int s = 0; s < parts; ++s) {
+    float l = 0.0f, o[E] = {};
+#pragma unroll 4
+    for (int s = warp; s < a.parts; s += 4) {
         const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (s * step + id));
         const float w = ex2(ml.x - ref);
         l += w * ml.y;
 #pragma unroll
-        for (int e = 0; e < D / 32; ++e) o[e] += w * a.part_o[(s * step + id) * D + lane * (D / 32) + e];
+        for (int e = 0; e < E; ++e) o[e] += w * a.part_o[(s * step + id) * D + lane * E + e];
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* dst = a.o + row * a.o_ld + h * a.o_hs + lane * (D / 32);
 #pragma unroll
-    for (int e = 0; e < D / 32; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(o[e] * inv, o[e + 1] * inv);
+    for (int e = 0; e < E; ++e) so[warp][lane * E + e] = o[e];
+    if (lane == 0) sl[warp] = l;
+    __syncthreads();
+    if (threadIdx.x < D / 2) {
+        const int ch = 2 * threadIdx.x;
+        const float total = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        float x[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) x[e] = ((so[0][ch + e] + so[1][ch + e]) + (so[2][ch + e] + so[3][ch + e])) * inv;
+        *reinterpret_cast<uint32_t*>(a.o + row * a.o_ld + h * a.o_hs + ch) = pack_bf16x2(x[0], x[1]);
+    }
 }
 
 // o = 0 where there is no key at all, 8 channels a thread.
@@ -802,7 +1042,19 @@ static int64_t parts_of(bool cache, int64_t nq, int64_t heads, int64_t steps) {
     return best;
 }
 
+// The same for the rows kernel: rounds of two CTAs an SM, whose warps take a
+// segment each at a time, plus about one segment's time for the rest of a CTA.
+static int64_t row_parts_of(int64_t tiles, int64_t segs) {
+    int64_t best = 1, best_cost = 0;
+    for (int64_t n = 1; n <= 64 && (n == 1 || n <= cdiv(segs, kRowWarps)); ++n) {
+        const int64_t cost = cdiv(tiles * n, 2 * sm_count()) * (cdiv(segs, n * kRowWarps) + 1) + (n > 1 ? 2 : 0);
+        if (n == 1 || cost < best_cost) best = n, best_cost = cost;
+    }
+    return best;
+}
+
 struct Plan {
+    bool rows;               // the rows kernel
     int64_t heads;           // heads a launch (and of the widened copy)
     int64_t parts;           // of the keys
     int64_t join_at, bytes;  // in the workspace
@@ -811,8 +1063,14 @@ struct Plan {
 constexpr int64_t kWideBytes = 256ll << 20;  // of widened heads at a time (one head at least)
 
 static Plan plan(bool cache, int64_t Sq, int64_t H, int64_t D, int64_t segs) {
-    Plan p{H, 1, 0, 0};
+    Plan p{false, H, 1, 0, 0};
     if (segs == 0) return p;
+    if (cache && Sq <= kRowsMost) {
+        p.rows = true;
+        p.parts = row_parts_of(cdiv(Sq, kFewRows) * H, segs);
+        p.bytes = p.parts > 1 ? p.parts * H * Sq * (D + 2) * 4 : 0;
+        return p;
+    }
     const int64_t nq = cdiv(Sq, kQRows);
     const int64_t head = cache ? 2 * segs * kSeg * D * 2 : 0;
     if (H * head > kWideBytes) p.heads = kWideBytes / head > 0 ? kWideBytes / head : 1;
@@ -836,7 +1094,7 @@ static int launch_pairs(Args a, const uint16_t* const (&kv)[2], const int64_t (&
     H3B_CUDA_TRY(cudaFuncSetAttribute(pair_kernel<D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes));
     const int64_t grid = items < sm_count() ? items : sm_count();
     pair_kernel<D, SRC><<<(unsigned)grid, kPairThreads, Smem<D>::kBytes, s>>>(q, k, v, o, a);
-    if (a.parts > 1) join_kernel<D><<<(unsigned)cdiv(a.Sq * a.heads, 4), 128, 0, s>>>(a, a.heads, a.parts);
+    if (a.parts > 1) join_kernel<D><<<(unsigned)(a.Sq * a.heads), 128, 0, s>>>(a);
     H3B_CUDA_TRY(cudaGetLastError());
     return H3B_OK;
 }
@@ -847,6 +1105,12 @@ static int launch_all(Args& a, bool cache, const Plan& p, char* ws, cudaStream_t
     a.part_ml = a.part_o + (p.parts > 1 ? p.parts * p.heads * a.Sq * D : 0);
     a.parts = (int)p.parts;
     a.heads = a.H;
+    if (p.rows) {
+        rows_kernel<D><<<(unsigned)(cdiv(a.Sq, kFewRows) * a.H * p.parts), 32 * kRowWarps, 0, s>>>(a);
+        if (p.parts > 1) join_kernel<D><<<(unsigned)(a.Sq * a.H), 128, 0, s>>>(a);
+        H3B_CUDA_TRY(cudaGetLastError());
+        return H3B_OK;
+    }
     if (!cache) return launch_pairs<D, kBlocks>(a, a.kv, a.kv_ld, a.kv_hs, s);
     const int64_t rows = a.segs * kSeg;
     uint16_t* const k = reinterpret_cast<uint16_t*>(ws);
@@ -880,7 +1144,7 @@ static int launch(const char* who, bool cache, Args& a, int64_t D, int64_t segs,
     a.segs = segs;
     a.nq = cdiv(a.Sq, kQRows);
     const Plan p = plan(cache, a.Sq, a.H, D, segs);
-    H3B_REQUIRE(a.nq * a.H * p.parts < (1ll << 30) && a.Sq * a.H < (1ll << 33), "%s: too many row tiles", who);
+    H3B_REQUIRE(a.nq * a.H * p.parts < (1ll << 28) && a.Sq * a.H < (1ll << 31), "%s: too many row tiles", who);
     H3B_REQUIRE(p.bytes == 0 || (ws && aligned(ws, 256) && ws_bytes >= p.bytes),
                 "%s: workspace of %lld bytes (256-byte aligned), %lld needed", who, (long long)ws_bytes, (long long)p.bytes);
     DeviceStatus ds;
