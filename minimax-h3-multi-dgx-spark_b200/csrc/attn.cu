@@ -1,6 +1,8 @@
 // Attention over a key/value cache held in 8 bits, and over selected blocks of
 // bf16 keys:  o = softmax(scale * q k^T) v, one pass over the keys with the
 // running maximum and sum of the softmax.
+#include <cuda_fp16.h>
+
 #include <type_traits>
 
 #include "ptx.cuh"
@@ -215,11 +217,6 @@ __device__ __forceinline__ uint32_t widen2(uint32_t t) {
 }
 // bytes 0 and 1 (sel 0x4140) or 2 and 3 (0x4342) of a word
 __device__ __forceinline__ uint32_t codes_to_bf16x2(uint32_t x, uint32_t sel) { return widen2(__byte_perm(x, 0, sel)); }
-// byte i of two words
-__device__ __forceinline__ uint32_t code_pair(uint32_t x, uint32_t y, int i) {
-    return widen2(__byte_perm(x, y, i | ((4 + i) << 8)));
-}
-
 // Where a tile's keys and values come from.
 enum Source {
     kBlocks,  // selected blocks of bf16 tensors, each tile its own
@@ -711,75 +708,127 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
 // ---------------------------------------------------------------------------
 // Rows kernel: few query rows over the cache.  The codes are read once, straight
-// into registers, and widened there as operands of mma.sync m16n8k16: 16 query
-// rows a warp, 16 keys a turn.  Which channel (of the scores) or key and channel
-// (of the output) an operand's register stands for is ours to choose, as long as
-// both operands agree, so every thread loads 16 (or 8) consecutive codes:
-//   scores   thread (g, c) = (lane / 4, lane % 4) holds D / 4 channels of keys
-//            4 (g / 2) + g % 2 and two behind it
-//   output   D / 8 channels of keys 4 c .. 4 c + 3
-// The scores' accumulators then are the output product's P operand as they lie.
-// What bounds it is the cache's bytes: 16 rows take about 2 instructions a clock
-// and SM at the rate at which HBM delivers them.
+// into registers, and widened there as the A operand of mma.sync m16n8k16 with
+// the query rows as its 8 columns (GROUPS times 8 rows a warp), 16 keys a turn:
+//   S^T = K Q^T   thread (g, c) = (lane / 4, lane % 4) holds D / 4 channels of
+//                 keys g and g + 8
+//   O^T = V^T P^T it holds D / 8 channels of keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9
+// (which channel an operand's register stands for is ours to choose), so a load
+// is 16 or 8 consecutive codes, and P^T is S^T's accumulators transposed 8 x 8.
+//
+// Operands are fp16, to which a code widens in fewer instructions than to bf16
+// (0x6400 | code + 128 is 1024 + code + 128): the codes are exact; a query row
+// is scaled by a power of two that brings its largest element to 2^14 (elements
+// are exact down to 2^-28 of it and off by 2^-39 of it below); p is taken 2^11
+// times larger and its reference moves at 2^4, so it stays below 2^15 and what
+// rounds to zero is below 2^-35 of the largest.  A block's value scale would
+// leave that range: each block's output is accumulated apart and joins O with it.
+//
+// What bounds it is the cache's bytes.  16 keys of 128 channels take about 270
+// instructions for 8 rows, 40% of what an SM can issue in the time that HBM
+// takes to deliver them.
 
-constexpr int kFewRows = 16;   // query rows a warp
 constexpr int kRowWarps = 4;   // of a CTA, each with its own segments
+constexpr float kRowSlack = 4.0f, kRowBias = 11.0f;
 // Up to this many rows the rows kernel reads the codes once per 16 rows (from L2
 // after the first); beyond, they are widened once for the pair kernel.
 constexpr int64_t kRowsMost = 64;
 
-__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Codes with their sign bit flipped, bytes 0 and 1 (or 2 and 3) of x -> fp16x2
+template <bool HIGH>
+__device__ __forceinline__ uint32_t half_codes(uint32_t x) {
+    const uint32_t t = __byte_perm(x, 0x64646464u, HIGH ? 0x4342 : 0x4140), base = 0x64806480u;  // 1024 + 128
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&t), *reinterpret_cast<const __half2*>(&base));
+    return *reinterpret_cast<const uint32_t*>(&d);
 }
 
-template <int D>
-__global__ void __launch_bounds__(32 * kRowWarps, 2) rows_kernel(const __grid_constant__ Args a) {
-    constexpr int kC = D / 4;        // channels of a thread's keys (scores)
-    constexpr int kN = D / 8;        // channels of a thread (output), and n-tiles of 8 channels
-    constexpr int kKW = kC / 16;     // uint4 a key
+// CTAs an SM: as many as the registers allow without spilling (three instead of
+// two: 0.248 ms instead of 0.302 for a row over 131071 tokens of 40 heads).
+constexpr int row_ctas(int64_t D, int groups) { return groups == 2 ? 2 : D == 128 ? 3 : 4; }
+
+template <int D, int GROUPS>
+__global__ void __launch_bounds__(32 * kRowWarps, row_ctas(D, GROUPS)) rows_kernel(const __grid_constant__ Args a) {
+    constexpr int kRows = 8 * GROUPS;
+    constexpr int kC = D / 4;     // channels of a thread's keys (scores)
+    constexpr int kN = D / 8;     // channels of a thread's keys (output)
+    constexpr int kKW = kC / 16;  // uint4 a key
+    constexpr int kNW = kN / 4;   // words a key (output)
     using Piece = typename std::conditional<D == 128, uint4, uint2>::type;  // kN codes
-    __shared__ float so[kRowWarps][kFewRows][D];
-    __shared__ float sm[kRowWarps][kFewRows], sl[kRowWarps][kFewRows];
+    __shared__ float so[kRowWarps][kRows][D];
+    __shared__ float sm[kRowWarps][kRows], sl[kRowWarps][kRows];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     // row groups first: CTAs that run together share a head's codes in L2
-    const uint32_t groups = (uint32_t)((a.Sq + kFewRows - 1) / kFewRows);
-    const uint32_t rest = blockIdx.x / groups;
-    const int64_t row0 = (int64_t)(blockIdx.x - rest * groups) * kFewRows;
+    const uint32_t tiles = (uint32_t)((a.Sq + kRows - 1) / kRows);
+    const uint32_t rest = blockIdx.x / tiles;
+    const int64_t row0 = (int64_t)(blockIdx.x - rest * tiles) * kRows;
     const int part = (int)(rest / (uint32_t)a.H), h = (int)(rest - part * (uint32_t)a.H);
-    const int rows = (int)min((int64_t)kFewRows, a.Sq - row0);
+    const int rows = (int)min((int64_t)kRows, a.Sq - row0);
 
-    uint32_t q[kC / 4][4];
+    // Q^T: row g of each group, channels kC c ..
+    uint32_t q[GROUPS][kC / 2];
+    float factor[GROUPS][2];  // of the scores of rows 2 c, 2 c + 1
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const uint16_t* src = a.q + (row0 + g + 8 * r) * a.q_ld + h * a.q_hs + c * kC;
+    for (int r = 0; r < GROUPS; ++r) {
+        const uint16_t* src = a.q + (row0 + 8 * r + g) * a.q_ld + h * a.q_hs + c * kC;
+        uint32_t top = 0;
 #pragma unroll
         for (int j = 0; j < kC / 8; ++j) {
             uint4 x = make_uint4(0, 0, 0, 0);
-            if (g + 8 * r < rows) x = *reinterpret_cast<const uint4*>(src + 8 * j);
-            q[2 * j][r] = x.x;
-            q[2 * j][r + 2] = x.y;
-            q[2 * j + 1][r] = x.z;
-            q[2 * j + 1][r + 2] = x.w;
+            if (8 * r + g < rows) x = *reinterpret_cast<const uint4*>(src + 8 * j);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                q[r][4 * j + e] = w[e];
+                top = max(top, max(w[e] & 0x7FFFu, (w[e] >> 16) & 0x7FFFu));
+            }
         }
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+        top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+        // exponent field of the largest element; 2^(14 - exponent) as long as that is a number, 1 beside an
+        // infinity or NaN
+        const int e = max((int)(top >> 7), 40);
+        const float up = e == 255 ? 1.0f : __int_as_float((127 + 14 + 127 - e) << 23);
+        const float down = e == 255 ? 1.0f : __int_as_float((127 - 14 - 127 + e) > 0 ? (e - 14) << 23 : 0);
+#pragma unroll
+        for (int j = 0; j < kC / 2; ++j) q[r][j] = pack_half2(bf16_lo(q[r][j]) * up, bf16_hi(q[r][j]) * up);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            factor[r][k] = a.scale * kLog2e * __shfl_sync(0xFFFFFFFFu, down, (2 * c + k) * 4);
     }
 
-    float o[kN][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    float o[GROUPS][kN / 2][4], m[GROUPS][2], l[GROUPS][2];
 #pragma unroll
-    for (int j = 0; j < kN; ++j)
+    for (int r = 0; r < GROUPS; ++r) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+        for (int j = 0; j < kN / 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[r][j][e] = 0.0f;
+        m[r][0] = m[r][1] = -INFINITY;
+        l[r][0] = l[r][1] = 0.0f;
+    }
 
     // this warp's segments: seg0, seg0 + kRowWarps, .. below seg1
-    const int64_t segs = a.segs, seg1 = segs * (part + 1) / a.parts;
-    const int64_t seg0 = segs * part / a.parts + warp;
-    const int8_t* kbase = a.codes[0] + ((int64_t)h * a.cap + 4 * (g >> 1) + (g & 1)) * D + c * kC;
-    const int8_t* vbase = a.codes[1] + ((int64_t)h * a.cap + 4 * c) * D + g * kN;
+    const int64_t seg1 = a.segs * (part + 1) / a.parts, seg0 = a.segs * part / a.parts + warp;
+    const int8_t* kbase = a.codes[0] + ((int64_t)h * a.cap + g) * D + c * kC;
+    const int8_t* vbase = a.codes[1] + ((int64_t)h * a.cap + 2 * c) * D + g * kN;
     const float* ks = a.scales[0] + (int64_t)h * (a.cap / kSeg);
     const float* vs = a.scales[1] + (int64_t)h * (a.cap / kSeg);
-    const float scale2 = a.scale * kLog2e;
     uint4 kx[2][kKW];
     Piece vx[4];
     auto fetch = [&](int64_t seg, int turn) {
@@ -787,10 +836,10 @@ __global__ void __launch_bounds__(32 * kRowWarps, 2) rows_kernel(const __grid_co
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int w = 0; w < kKW; ++w)
-                kx[t][w] = __ldcs(reinterpret_cast<const uint4*>(kbase + at + t * 2 * D) + w);
+            for (int w = 0; w < kKW; ++w) kx[t][w] = __ldcs(reinterpret_cast<const uint4*>(kbase + at + t * 8 * D) + w);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) vx[k] = __ldcs(reinterpret_cast<const Piece*>(vbase + at + k * D));
+        for (int k = 0; k < 4; ++k)
+            vx[k] = __ldcs(reinterpret_cast<const Piece*>(vbase + at + ((k & 1) + (k & 2) * 4) * D));
     };
     float sk = 0.0f, sv = 0.0f;
     if (seg0 < seg1) {
@@ -799,112 +848,127 @@ __global__ void __launch_bounds__(32 * kRowWarps, 2) rows_kernel(const __grid_co
         sv = __ldg(vs + seg0);
     }
     for (int64_t seg = seg0; seg < seg1; seg += kRowWarps) {
-        const float fk = sk * scale2, fv = sv;
+        const float fk = sk, fv = sv;
         const int valid = (int)min((int64_t)kSeg, a.keys - seg * kSeg);
         const bool more = seg + kRowWarps < seg1;
         if (more) {
             sk = __ldg(ks + seg + kRowWarps);
             sv = __ldg(vs + seg + kRowWarps);
         }
+        float os[GROUPS][kN / 2][4];  // this block's output, without its scale
+#pragma unroll
+        for (int r = 0; r < GROUPS; ++r)
+#pragma unroll
+            for (int j = 0; j < kN / 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) os[r][j][e] = 0.0f;
 #pragma unroll 1
         for (int turn = 0; turn < kSeg / 16; ++turn) {
-            uint4 kc[2][kKW];
-            Piece vc[4];
+            uint32_t kc[2][kC / 4], vc[4][kNW];
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int w = 0; w < kKW; ++w) kc[t][w] = kx[t][w];
+                for (int w = 0; w < kC / 4; ++w) kc[t][w] = reinterpret_cast<const uint32_t*>(kx[t])[w] ^ 0x80808080u;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) vc[k] = vx[k];
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int w = 0; w < kNW; ++w) vc[k][w] = reinterpret_cast<const uint32_t*>(&vx[k])[w] ^ 0x80808080u;
             if (turn + 1 < kSeg / 16) fetch(seg, turn + 1);
             else if (more) fetch(seg + kRowWarps, 0);
-            // scores: two n-tiles, of keys 4 c, 4 c + 1 and of keys 4 c + 2, 4 c + 3 in this thread
-            float s[2][4] = {};
+            float s[GROUPS][4];
 #pragma unroll
-            for (int j = 0; j < kC / 4; ++j)
+            for (int r = 0; r < GROUPS; ++r) s[r][0] = s[r][1] = s[r][2] = s[r][3] = 0.0f;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const uint4 x = kc[t][j / 4];
-                    const uint32_t w = j % 4 == 0 ? x.x : j % 4 == 1 ? x.y : j % 4 == 2 ? x.z : x.w;
-                    mma_16816(s[t], q[j], codes_to_bf16x2(w, 0x4140), codes_to_bf16x2(w, 0x4342));
-                }
-            const int left = valid - turn * 16 - 4 * c;  // of this thread's four keys
-            float x[2][4];                               // [row half][key]
+            for (int j = 0; j < kC / 4; ++j) {
+                const uint32_t a0 = half_codes<false>(kc[0][j]), a1 = half_codes<false>(kc[1][j]),
+                               a2 = half_codes<true>(kc[0][j]), a3 = half_codes<true>(kc[1][j]);
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float y = s[k >> 1][2 * r + (k & 1)] * fk;
-                    x[r][k] = k < left ? y : -INFINITY;
-                }
-            float top[2];
+                for (int r = 0; r < GROUPS; ++r) mma_16816(s[r], a0, a1, a2, a3, q[r][2 * j], q[r][2 * j + 1]);
+            }
+            // s[r][2 t + k]: key g + 8 t, row 2 c + k
+            const int left = valid - turn * 16 - g;
             bool moves = false;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                top[r] = fmaxf(fmaxf(x[r][0], x[r][1]), fmaxf(x[r][2], x[r][3]));
-                moves |= top[r] > m[r] + kSlack || (m[r] == -INFINITY && top[r] > m[r]);
-            }
+            for (int r = 0; r < GROUPS; ++r)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[r][e] = (e < 2 ? 0 : 8) < left ? s[r][e] * (fk * factor[r][e & 1]) : -INFINITY;
+                    moves |= s[r][e] > m[r][e & 1] + kRowSlack || (m[r][e & 1] == -INFINITY && s[r][e] > -INFINITY);
+                }
             if (__any_sync(0xFFFFFFFFu, moves)) {
-                float keep[2];
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 1));
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], 2));
-                    const float to = fmaxf(m[r], top[r]);
-                    keep[r] = to == m[r] ? 1.0f : ex2(m[r] - to);
-                    m[r] = to;
-                    l[r] *= keep[r];
-                }
+                for (int r = 0; r < GROUPS; ++r) {
+                    float keep[2];
 #pragma unroll
-                for (int j = 0; j < kN; ++j) {
-                    o[j][0] *= keep[0];
-                    o[j][1] *= keep[0];
-                    o[j][2] *= keep[1];
-                    o[j][3] *= keep[1];
+                    for (int k = 0; k < 2; ++k) {
+                        float top = fmaxf(s[r][k], s[r][2 + k]);
+#pragma unroll
+                        for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
+                        const float to = fmaxf(m[r][k], top);
+                        keep[k] = to == m[r][k] ? 1.0f : ex2(m[r][k] - to);
+                        m[r][k] = to;
+                        l[r][k] *= keep[k];
+                    }
+#pragma unroll
+                    for (int j = 0; j < kN / 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            o[r][j][e] *= keep[e & 1];
+                            os[r][j][e] *= keep[e & 1];
+                        }
                 }
             }
-            uint32_t p[4];
+            uint32_t p[GROUPS][2];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const float ref = m[r] == -INFINITY ? 0.0f : m[r];
+            for (int r = 0; r < GROUPS; ++r) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    x[r][k] = ex2(x[r][k] - ref);
-                    l[r] += x[r][k];
-                    x[r][k] *= fv;
+                for (int e = 0; e < 4; ++e) {
+                    const float ref = m[r][e & 1] == -INFINITY ? 0.0f : m[r][e & 1] - kRowBias;
+                    s[r][e] = ex2(s[r][e] - ref);
+                    l[r][e & 1] += s[r][e];
                 }
-                // p is rounded to bf16 for the second product (its sum is not): a relative 2^-8 at most a key
-                p[r] = pack_bf16x2(x[r][0], x[r][1]);
-                p[r + 2] = pack_bf16x2(x[r][2], x[r][3]);
+                // p is rounded to fp16 for the second product (its sum is not): a relative 2^-11 at most a key
+                p[r][0] = transpose_8x8(pack_half2(s[r][0], s[r][1]));
+                p[r][1] = transpose_8x8(pack_half2(s[r][2], s[r][3]));
             }
-            // output: n-tile j has channel kN g + j in this thread, whose keys are bytes of four different words
+            // tile j has channels kN g + 2 j and 2 j + 1 of this thread, whose keys are bytes of four words
 #pragma unroll
-            for (int j = 0; j < kN; ++j) {
-                uint32_t w[4];
+            for (int w = 0; w < kNW; ++w)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) w[k] = reinterpret_cast<const uint32_t*>(&vc[k])[j / 4];
-                mma_16816(o[j], p, code_pair(w[0], w[1], j % 4), code_pair(w[2], w[3], j % 4));
-            }
+                for (int half = 0; half < 2; ++half) {
+                    const int sel = half ? 0x7362 : 0x5140;
+                    const uint32_t x = __byte_perm(vc[0][w], vc[1][w], sel), y = __byte_perm(vc[2][w], vc[3][w], sel);
+                    const uint32_t a0 = half_codes<false>(x), a1 = half_codes<true>(x), a2 = half_codes<false>(y),
+                                   a3 = half_codes<true>(y);
+#pragma unroll
+                    for (int r = 0; r < GROUPS; ++r) mma_16816(os[r][2 * w + half], a0, a1, a2, a3, p[r][0], p[r][1]);
+                }
         }
+#pragma unroll
+        for (int r = 0; r < GROUPS; ++r)
+#pragma unroll
+            for (int j = 0; j < kN / 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[r][j][e] = fmaf(os[r][j][e], fv, o[r][j][e]);
     }
     // the warps' parts meet in shared memory
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], 2);
-        if (c == 0) {
-            sm[warp][g + 8 * r] = m[r];
-            sl[warp][g + 8 * r] = l[r];
-        }
-        // accumulator columns 2 c, 2 c + 1 of n-tile j are its rows' channels kN (2 c) + j and kN (2 c + 1) + j
-        if (g + 8 * r < rows) {
+    for (int r = 0; r < GROUPS; ++r)
 #pragma unroll
-            for (int j = 0; j < kN; ++j) {
-                so[warp][g + 8 * r][kN * 2 * c + j] = o[j][2 * r];
-                so[warp][g + 8 * r][kN * (2 * c + 1) + j] = o[j][2 * r + 1];
+        for (int k = 0; k < 2; ++k) {
+            const int row = 8 * r + 2 * c + k;
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) l[r][k] += __shfl_xor_sync(0xFFFFFFFFu, l[r][k], off);
+            if (g == 0) {
+                sm[warp][row] = m[r][k];
+                sl[warp][row] = l[r][k];
+            }
+            if (row < rows) {
+#pragma unroll
+                for (int j = 0; j < kN / 2; ++j)
+                    *reinterpret_cast<float2*>(&so[warp][row][kN * g + 2 * j]) = make_float2(o[r][j][k], o[r][j][2 + k]);
             }
         }
-    }
     __syncthreads();
     for (int e = threadIdx.x; e < rows * (D / 2); e += 32 * kRowWarps) {
         const int r = e / (D / 2), ch = 2 * (e % (D / 2));
@@ -1042,12 +1106,12 @@ static int64_t parts_of(bool cache, int64_t nq, int64_t heads, int64_t steps) {
     return best;
 }
 
-// The same for the rows kernel: rounds of two CTAs an SM, whose warps take a
+// The same for the rows kernel: rounds of the CTAs that fit, whose warps take a
 // segment each at a time, plus about one segment's time for the rest of a CTA.
-static int64_t row_parts_of(int64_t tiles, int64_t segs) {
+static int64_t row_parts_of(int64_t tiles, int64_t segs, int ctas) {
     int64_t best = 1, best_cost = 0;
     for (int64_t n = 1; n <= 64 && (n == 1 || n <= cdiv(segs, kRowWarps)); ++n) {
-        const int64_t cost = cdiv(tiles * n, 2 * sm_count()) * (cdiv(segs, n * kRowWarps) + 1) + (n > 1 ? 2 : 0);
+        const int64_t cost = cdiv(tiles * n, ctas * sm_count()) * (cdiv(segs, n * kRowWarps) + 1) + (n > 1 ? 2 : 0);
         if (n == 1 || cost < best_cost) best = n, best_cost = cost;
     }
     return best;
@@ -1067,7 +1131,8 @@ static Plan plan(bool cache, int64_t Sq, int64_t H, int64_t D, int64_t segs) {
     if (segs == 0) return p;
     if (cache && Sq <= kRowsMost) {
         p.rows = true;
-        p.parts = row_parts_of(cdiv(Sq, kFewRows) * H, segs);
+        const int groups = Sq <= 8 ? 1 : 2;
+        p.parts = row_parts_of(cdiv(Sq, 8 * groups) * H, segs, row_ctas(D, groups));
         p.bytes = p.parts > 1 ? p.parts * H * Sq * (D + 2) * 4 : 0;
         return p;
     }
@@ -1106,7 +1171,8 @@ static int launch_all(Args& a, bool cache, const Plan& p, char* ws, cudaStream_t
     a.parts = (int)p.parts;
     a.heads = a.H;
     if (p.rows) {
-        rows_kernel<D><<<(unsigned)(cdiv(a.Sq, kFewRows) * a.H * p.parts), 32 * kRowWarps, 0, s>>>(a);
+        if (a.Sq <= 8) rows_kernel<D, 1><<<(unsigned)(a.H * p.parts), 32 * kRowWarps, 0, s>>>(a);
+        else rows_kernel<D, 2><<<(unsigned)(cdiv(a.Sq, 16) * a.H * p.parts), 32 * kRowWarps, 0, s>>>(a);
         if (p.parts > 1) join_kernel<D><<<(unsigned)(a.Sq * a.H), 128, 0, s>>>(a);
         H3B_CUDA_TRY(cudaGetLastError());
         return H3B_OK;

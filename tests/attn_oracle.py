@@ -23,14 +23,16 @@ def softmax_rows(q, k, v, scale, seen=None):
     return p @ v, p @ v.abs(), m
 
 
-def tolerance(o, a, m, n, d):
+def tolerance(o, a, m, n, d, vsum=0.0):
     """Bound on |kernel - o|: the result's rounding to bf16, and, relative to a = sum p |v|: p's rounding to bf16
     before the second product; scores as sums of d products and two factors in fp32, an absolute error of
     (d + 4) 2^-24 m each that moves p and the sum of p by as much; the exponential (2^-20 covers ex2.approx and the
     rounding of its argument at |argument| < 8; larger arguments come with an m that covers them); sums over n keys in
-    fp32."""
+    fp32.  vsum, the sum of |v| over the keys, where p may be rounded to fp16 instead: relative 2^-11, which 2^-8 covers,
+    but no less than half of fp16's smallest step, 2^-25.  p is 2^11 there for the key that set the row's reference, so
+    the sum of p is 2^11 at least and a weight is off by 2^-36 at most: vsum 2^-36 together."""
     return BF16_HALF * (o.abs() + a * (1 + 2.0 ** -7)) + a * (2 * (d + 4) * F32_HALF * m + 2.0 ** -20 + 2 * n * F32_HALF) \
-        + 1e-30
+        + vsum * 2.0 ** -36 + 1e-30
 
 
 def quantise(x, codes, scales, start):
