@@ -317,6 +317,18 @@ H3B_API int h3b_block_sparse_attn(const void *q, int64_t q_ld, int64_t q_hs, int
                                   void *o, int64_t o_ld, int64_t o_hs, void *workspace, int64_t workspace_bytes,
                                   void *stream);
 
+/* The four steps above in one call: means of 64 keys (unless the caller keeps
+ * them: k_means fp32 [ceil(Sk / 64), H, D], or NULL) and of 128 query rows, the
+ * min(topk, ceil(Sk / 64)) blocks of each head and query block -> blocks int32
+ * [H, ceil(Sq / 128), that many], and the attention over them -> o.  Workspace as
+ * h3b_sparse_attn_workspace says (256-byte aligned).  In place of the
+ * scaled_dot_product_attention of sp_forward.py:276-318. */
+H3B_API int64_t h3b_sparse_attn_workspace(int64_t Sq, int64_t Sk, int64_t H, int64_t D, int64_t topk, int has_means);
+H3B_API int h3b_sparse_attn(const void *q, int64_t q_ld, int64_t q_hs, int64_t Sq, int64_t H, int64_t D, const void *k,
+                            int64_t k_ld, int64_t k_hs, const void *v, int64_t v_ld, int64_t v_hs, int64_t Sk,
+                            const float *k_means, int64_t topk, float scale, int32_t *blocks, void *o, int64_t o_ld,
+                            int64_t o_hs, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* ---- Ulysses all-to-all -------------------------------------------------- */
 
 /* Forward pack: rows of t (row stride t_ld bytes) hold one block of

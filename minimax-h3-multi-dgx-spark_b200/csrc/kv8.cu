@@ -12,7 +12,7 @@
 // A non-finite x makes the scale non-finite and the block's codes 0, so
 // everything read from it is NaN.  Maxima run on the bit patterns of |x|,
 // which order NaN above infinity above the numbers.
-#include "common.cuh"
+#include "quant_common.cuh"
 
 namespace h3b {
 namespace kv8 {
@@ -28,16 +28,6 @@ struct WriteArgs {
     int64_t cap, start, n;
     int H;
 };
-
-__device__ __forceinline__ uint32_t abs_bits(uint32_t bf16x2, int half) {
-    return half ? (bf16x2 & 0x7FFF0000u) : ((bf16x2 << 16) & 0x7FFF0000u);
-}
-
-__device__ __forceinline__ int quant1(float x, float s, bool live) {
-    if (!live) return 0;
-    const float r = rintf(__fdiv_rn(x, s));
-    return (int)fminf(fmaxf(r, -127.0f), 127.0f);
-}
 
 __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
     return (uint32_t)(a & 255) | ((uint32_t)(b & 255) << 8) | ((uint32_t)(c & 255) << 16) | ((uint32_t)(d & 255) << 24);
@@ -60,7 +50,7 @@ __global__ void __launch_bounds__(kThreads) write_kernel(WriteArgs a) {
     float* scale = a.scales[which] + (int64_t)h * (a.cap / kBlock) + b;
 
     uint4 v[kPasses];
-    uint32_t top = 0;
+    uint32_t pair = 0;  // maxima of the low and of the high halves' bits
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
         const int64_t t = b * kBlock + row + p * kRows;
@@ -70,12 +60,10 @@ __global__ void __launch_bounds__(kThreads) write_kernel(WriteArgs a) {
     }
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
-        const uint32_t w[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top = max(top, max(abs_bits(w[e], 0), abs_bits(w[e], 1)));
+        pair = absmax_bits8(v[p], pair);
     }
     __shared__ uint32_t tops[kThreads / 32];
-    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(fold_absmax_bits(pair)));
     if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
     const bool stays = a.start > b * kBlock;  // older tokens in this block
     const float older = stays ? *scale : 0.0f;
@@ -86,6 +74,7 @@ __global__ void __launch_bounds__(kThreads) write_kernel(WriteArgs a) {
     float s = __fdiv_rn(__uint_as_float(top), 127.0f);
     if ((__float_as_uint(older) & 0x7FFFFFFFu) > (__float_as_uint(s) & 0x7FFFFFFFu)) s = older;
     const bool live = s > 0.0f && s < __int_as_float(0x7F800000);
+    const float inverse = live ? __frcp_rn(s) : 0.0f;
     const bool grew = stays && __float_as_uint(s) != __float_as_uint(older);
     const float ratio = grew && live ? __fdiv_rn(older, s) : 0.0f;
 #pragma unroll
@@ -95,14 +84,10 @@ __global__ void __launch_bounds__(kThreads) write_kernel(WriteArgs a) {
         if (t >= end) continue;
         uint2* dst = reinterpret_cast<uint2*>(codes + (int64_t)r * D);
         if (t >= a.start) {
-            const uint32_t w[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
-            int c[8];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                c[2 * e] = quant1(bf16_lo(w[e]), s, live);
-                c[2 * e + 1] = quant1(bf16_hi(w[e]), s, live);
-            }
-            *dst = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+            float x[8];
+            unpack8(v[p], x);
+            // (the scale is the block's absmax / 127 or larger, so no code leaves [-127, 127])
+            *dst = live ? quant8(x, s, inverse) : make_uint2(0u, 0u);
         } else if (grew) {
             const uint2 old = *dst;
             int c[8];

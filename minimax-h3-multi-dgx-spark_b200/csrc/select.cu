@@ -15,84 +15,133 @@ constexpr int kThreads = 256;
 
 // mean over the rows of a block of x [S, H, D] -> out [nb, H, D] fp32.
 // One CTA per (block, head); 8 channels a thread, kThreads / (D / 8) row lanes.
-template <int D>
+// Bound by its reads; a whole block's loads are all in flight before the first
+// conversion to 64 bits.
+template <int D, int ROWS>
 __global__ void __launch_bounds__(kThreads) means_kernel(const uint16_t* __restrict__ x, int64_t ld, int64_t hs,
-                                                         int64_t S, int H, int rows, float* __restrict__ out) {
+                                                         int64_t S, int H, float* __restrict__ out) {
     constexpr int kCols = D / 8;
     constexpr int kRows = kThreads / kCols;
+    constexpr int kLoads = ROWS / kRows;
+    constexpr int kWarps = kThreads / 32;
     const int h = (int)(blockIdx.x % (unsigned)H);
     const int64_t b = blockIdx.x / (unsigned)H;
     const int col = threadIdx.x % kCols, row = threadIdx.x / kCols;
-    const int count = (int)min((int64_t)rows, S - b * rows);
-    const uint16_t* src = x + b * rows * ld + h * hs + col * 8;
+    const int count = (int)min((int64_t)ROWS, S - b * ROWS);
+    const uint16_t* src = x + (b * ROWS + row) * ld + h * hs + col * 8;
+    uint4 v[kLoads];
+#pragma unroll
+    for (int p = 0; p < kLoads; ++p) {
+        v[p] = make_uint4(0, 0, 0, 0);
+        if (row + p * kRows < count) v[p] = __ldcs(reinterpret_cast<const uint4*>(src + (int64_t)p * kRows * ld));
+    }
     double acc[8] = {};
-#pragma unroll 4
-    for (int r = row; r < count; r += kRows) {
-        const uint4 v = *reinterpret_cast<const uint4*>(src + r * ld);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int p = 0; p < kLoads; ++p) {
+        const uint32_t w[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             acc[2 * e] += (double)bf16_lo(w[e]);
             acc[2 * e + 1] += (double)bf16_hi(w[e]);
         }
     }
-    __shared__ double part[kRows][D + 1];
+    // the row lanes of a warp, then the warps
+    __shared__ double part[kWarps][D];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) part[row][col * 8 + e] = acc[e];
+    for (int e = 0; e < 8; ++e) {
+#pragma unroll
+        for (int off = kCols; off < 32; off <<= 1) acc[e] += __shfl_xor_sync(0xFFFFFFFFu, acc[e], off);
+        if (threadIdx.x % 32 < kCols) part[threadIdx.x / 32][col * 8 + e] = acc[e];
+    }
     __syncthreads();
     if (threadIdx.x < D) {
         double t = 0.0;
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) t += part[r][threadIdx.x];
+        for (int w = 0; w < kWarps; ++w) t += part[w][threadIdx.x];
         out[(b * H + h) * D + threadIdx.x] = (float)(t / (double)count);
     }
 }
 
-constexpr int kTile = 64;   // query rows (and key blocks) per score tile
-constexpr int kDepth = 16;  // channels per step
+constexpr int kTile = 64;  // query rows (and key blocks) per score tile
+constexpr int kFew = 4;    // query blocks up to which the scores are plain products
 
 // score[unit][i][j] = sum_d qm[i, h, d] * km[j, h, d] in 64 bits, one unit
-// being 64 query blocks of a head.  256 threads, 4 x 4 scores each.
-__global__ void __launch_bounds__(256) score_kernel(const float* __restrict__ qm, const float* __restrict__ km,
-                                                    int nq, int64_t nk, int H, int D, int tiles, int64_t unit0,
+// being 64 query blocks of a head.  Four warps a tile of 64 x 64, each 32 x 32 by
+// mma.sync m8n8k4 in fp64; both operands lie in shared memory as fp32, their
+// whole depth at once.  Bound by the fp64 products.
+template <int D>
+__global__ void __launch_bounds__(128) score_kernel(const float* __restrict__ qm, const float* __restrict__ km, int nq,
+                                                    int64_t nk, int H, int tiles, int64_t unit0,
                                                     double* __restrict__ score) {
-    __shared__ double qs[kDepth][kTile + 1];
-    __shared__ double ks[kDepth][kTile + 1];
+    constexpr int kLd = D + 4;  // 8 rows x 4 channels of an operand meet 32 banks
+    extern __shared__ __align__(16) float tile[];
+    float *qs = tile, *ks = tile + kTile * kLd;
     const int64_t unit = unit0 + blockIdx.y;
     const int h = (int)(unit / tiles);
-    const int64_t i0 = (unit % tiles) * kTile;
-    const int64_t j0 = (int64_t)blockIdx.x * kTile;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    double acc[4][4] = {};
-    for (int d0 = 0; d0 < D; d0 += kDepth) {
-        for (int e = threadIdx.x; e < kTile * kDepth; e += 256) {
-            const int d = e % kDepth, r = e / kDepth;
-            qs[d][r] = i0 + r < nq ? (double)qm[((i0 + r) * H + h) * D + d0 + d] : 0.0;
-            ks[d][r] = j0 + r < nk ? (double)km[((j0 + r) * H + h) * D + d0 + d] : 0.0;
+    const int64_t i0 = (unit % tiles) * kTile, j0 = (int64_t)blockIdx.x * kTile;
+    for (int e = threadIdx.x; e < kTile * (D / 4); e += 128) {
+        const int r = e / (D / 4), d = e % (D / 4) * 4;
+        float4 x = make_float4(0, 0, 0, 0), y = x;
+        if (i0 + r < nq) x = *reinterpret_cast<const float4*>(qm + ((i0 + r) * H + h) * D + d);
+        if (j0 + r < nk) y = *reinterpret_cast<const float4*>(km + ((j0 + r) * H + h) * D + d);
+        *reinterpret_cast<float4*>(qs + r * kLd + d) = x;
+        *reinterpret_cast<float4*>(ks + r * kLd + d) = y;
+    }
+    __syncthreads();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int wi = (warp >> 1) * 32, wj = (warp & 1) * 32;
+    const float* qa = qs + (wi + (lane >> 2)) * kLd + (lane & 3);
+    const float* ka = ks + (wj + (lane >> 2)) * kLd + (lane & 3);
+    double acc[4][4][2] = {};
+#pragma unroll 4
+    for (int d = 0; d < D; d += 4) {
+        double x[4], y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[e] = (double)qa[e * 8 * kLd + d];
+            y[e] = (double)ka[e * 8 * kLd + d];
         }
-        __syncthreads();
 #pragma unroll
-        for (int d = 0; d < kDepth; ++d) {
-            double a[4], b[4];
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                a[e] = qs[d][ty + 16 * e];
-                b[e] = ks[d][tx + 16 * e];
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int f = 0; f < 4; ++f) acc[e][f] = fma(a[e], b[f], acc[e][f]);
-        }
-        __syncthreads();
+            for (int f = 0; f < 4; ++f)
+                asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
+                    : "+d"(acc[e][f][0]), "+d"(acc[e][f][1])
+                    : "d"(x[e]), "d"(y[f]));
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int f = 0; f < 4; ++f) {
-            const int64_t j = j0 + tx + 16 * f;
-            if (j < nk) score[((int64_t)blockIdx.y * kTile + ty + 16 * e) * nk + j] = acc[e][f];
-        }
+        for (int f = 0; f < 4; ++f)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int64_t j = j0 + wj + 8 * f + 2 * (lane & 3) + k;
+                if (j < nk) score[((int64_t)blockIdx.y * kTile + wi + 8 * e + (lane >> 2)) * nk + j] = acc[e][f][k];
+            }
+}
+
+// The same for up to kFew query blocks: one warp a key block, so that the means
+// of the keys are read once at full width.
+template <int D>
+__global__ void __launch_bounds__(kThreads) score_few_kernel(const float* __restrict__ qm, const float* __restrict__ km,
+                                                             int nq, int64_t nk, int H, int64_t unit0,
+                                                             double* __restrict__ score) {
+    constexpr int E = D / 32;
+    const int lane = threadIdx.x & 31;
+    const int64_t j = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    const int h = (int)(unit0 + blockIdx.y);
+    if (j >= nk) return;
+    double y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = (double)km[(j * H + h) * D + lane + 32 * e];
+    for (int i = 0; i < nq; ++i) {
+        double t = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) t = fma((double)qm[((int64_t)i * H + h) * D + lane + 32 * e], y[e], t);
+#pragma unroll
+        for (int off = 16; off; off >>= 1) t += __shfl_xor_sync(0xFFFFFFFFu, t, off);
+        if (lane == 0) score[((int64_t)blockIdx.y * kTile + i) * nk + j] = t;
+    }
 }
 
 // Unsigned key in the order of the scores: NaN lowest, -0 with +0.
@@ -103,68 +152,138 @@ __device__ __forceinline__ uint64_t sort_key(double s) {
 }
 
 // One CTA per (head, query block): radix selection of the topk-th largest key,
-// eight bits a pass, then the chosen indices in ascending order.
+// eight bits a pass until all keys that share the digits so far are taken, then
+// the chosen indices in ascending order.  A thread has consecutive keys: HELD of
+// them in registers, or as many as it takes, read again every pass (HELD 0).
+template <int HELD>
 __global__ void __launch_bounds__(kThreads) topk_kernel(const double* __restrict__ score, int nq, int64_t nk, int tiles,
-                                                        int64_t unit0, int topk, int32_t* __restrict__ blocks) {
+                                                        int64_t unit0, int topk, int per, int32_t* __restrict__ blocks) {
+    constexpr int kWarps = kThreads / 32;
     __shared__ int hist[256];
-    __shared__ uint64_t s_prefix;
-    __shared__ int s_want;
-    __shared__ int warp_n[kThreads / 32][2];
-    const int64_t unit = unit0 + blockIdx.x / kTile;
-    const int h = (int)(unit / tiles);
-    const int64_t i = (unit % tiles) * kTile + blockIdx.x % kTile;
+    __shared__ int s_digit, s_left, s_count;
+    __shared__ int warp_n[kWarps][2];
+    const int64_t unit = unit0 + blockIdx.x / per;
+    const int h = (int)(unit / tiles), r = blockIdx.x % per;  // `per` rows of a unit are in the launch
+    const int64_t i = (unit % tiles) * kTile + r;
     if (i >= nq) return;
-    const double* row = score + (int64_t)blockIdx.x * nk;
+    const double* row = score + ((int64_t)(blockIdx.x / per) * kTile + r) * nk;
     int32_t* out = blocks + ((int64_t)h * nq + i) * topk;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (topk == nk) {
+        for (int64_t j = threadIdx.x; j < nk; j += kThreads) out[j] = (int32_t)j;
+        return;
+    }
+    const int mine = HELD > 0 ? HELD : (int)((nk + kThreads - 1) / kThreads);
+    const int64_t j0 = (int64_t)threadIdx.x * mine;
+    uint64_t held[HELD > 0 ? HELD : 1];
+    if constexpr (HELD > 0) {
+#pragma unroll
+        for (int t = 0; t < HELD; ++t) held[t] = j0 + t < nk ? sort_key(row[j0 + t]) : 0;
+    }
+    auto each = [&](auto&& f) {
+        if constexpr (HELD > 0) {
+#pragma unroll
+            for (int t = 0; t < HELD; ++t) f(j0 + t, held[t]);
+        } else {
+            for (int t = 0; t < mine; ++t) f(j0 + t, j0 + t < nk ? sort_key(row[j0 + t]) : 0);
+        }
+    };
     uint64_t prefix = 0;
     int want = topk;  // how many are still to be taken among the keys with this prefix
-    for (int shift = 56; shift >= 0; shift -= 8) {
+    int shift = 56;
+    for (;; shift -= 8) {
         hist[threadIdx.x] = 0;
         __syncthreads();
-        for (int64_t j = threadIdx.x; j < nk; j += kThreads) {
-            const uint64_t key = sort_key(row[j]);
-            if (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1);
-        }
+        each([&](int64_t j, uint64_t key) {
+            // many keys share their leading digits: one addition for a warp's equal ones
+            const bool in = j < nk && (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8)));
+            const uint32_t digit = in ? (uint32_t)(key >> shift) & 255u : 256u;
+            const uint32_t same = __match_any_sync(0xFFFFFFFFu, digit);
+            if (in && lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
+        });
         __syncthreads();
-        if (threadIdx.x == 0) {
-            int left = want, digit = 255;
-            while (digit > 0 && hist[digit] < left) left -= hist[digit--];
-            s_prefix = prefix | ((uint64_t)digit << shift);
-            s_want = left;
-        }
-        __syncthreads();
-        prefix = s_prefix;
-        want = s_want;
-        __syncthreads();
-    }
-    // every key above `prefix` is taken, and the first `want` equal to it
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int above = 0, equal = 0;  // so far, before this round's
-    for (int64_t j0 = 0; j0 < nk; j0 += kThreads) {
-        const int64_t j = j0 + threadIdx.x;
-        const uint64_t key = j < nk ? sort_key(row[j]) : 0;
-        const bool gt = j < nk && key > prefix, eq = j < nk && key == prefix;
-        const uint32_t mg = __ballot_sync(0xFFFFFFFFu, gt), me = __ballot_sync(0xFFFFFFFFu, eq);
-        if (lane == 0) {
-            warp_n[warp][0] = __popc(mg);
-            warp_n[warp][1] = __popc(me);
-        }
-        __syncthreads();
-        int g = above, q = equal;
-        for (int w = 0; w < kThreads / 32; ++w) {
-            if (w < warp) {
-                g += warp_n[w][0];
-                q += warp_n[w][1];
+        if (warp == 0) {
+            // digits 255 - 8 lane downwards: the one in which the want-th largest lies
+            int n[8], sum = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                n[e] = hist[255 - 8 * lane - e];
+                sum += n[e];
             }
-            above += warp_n[w][0];
-            equal += warp_n[w][1];
+            int above = sum;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int y = __shfl_up_sync(0xFFFFFFFFu, above, off);
+                if (lane >= off) above += y;
+            }
+            above -= sum;  // keys with a larger digit than this lane's
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (above < want && want <= above + n[e]) {
+                    s_digit = 255 - 8 * lane - e;
+                    s_left = want - above;
+                    s_count = n[e];
+                }
+                above += n[e];
+            }
         }
-        const uint32_t below = (1u << lane) - 1u;
-        g += __popc(mg & below);
-        q += __popc(me & below);
-        if (gt || (eq && q < want)) out[g + min(q, want)] = (int32_t)j;
         __syncthreads();
+        prefix |= (uint64_t)s_digit << shift;
+        want = s_left;
+        const bool all = s_count == want;
+        __syncthreads();
+        if (all || shift == 0) break;
     }
+    // every key above the prefix is taken, and the first `want` that have it
+    int gt = 0, eq = 0;
+    each([&](int64_t j, uint64_t key) {
+        const uint64_t head = key >> shift;
+        gt += j < nk && head > (prefix >> shift);
+        eq += j < nk && head == (prefix >> shift);
+    });
+    int g = gt, q = eq;  // scanned over the threads before
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const int x = __shfl_up_sync(0xFFFFFFFFu, g, off), y = __shfl_up_sync(0xFFFFFFFFu, q, off);
+        if (lane >= off) g += x, q += y;
+    }
+    if (lane == 31) {
+        warp_n[warp][0] = g;
+        warp_n[warp][1] = q;
+    }
+    __syncthreads();
+    g -= gt;
+    q -= eq;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+        if (w < warp) {
+            g += warp_n[w][0];
+            q += warp_n[w][1];
+        }
+    each([&](int64_t j, uint64_t key) {
+        const uint64_t head = key >> shift;
+        if (j >= nk || head < (prefix >> shift)) return;
+        const bool equal = head == (prefix >> shift);
+        if (!equal || q < want) out[g + min(q, want)] = (int32_t)j;
+        g += !equal;
+        q += equal;
+    });
+}
+
+template <int D>
+static int scores(const float* qm, const float* km, int nq, int64_t nk, int H, int tiles, int64_t unit, int64_t units,
+                  double* score, cudaStream_t s) {
+    if (nq <= kFew) {
+        const dim3 grid((unsigned)cdiv(nk, kThreads / 32), (unsigned)units);
+        score_few_kernel<D><<<grid, kThreads, 0, s>>>(qm, km, nq, nk, H, unit, score);
+    } else {
+        constexpr int smem = 2 * kTile * (D + 4) * 4;
+        H3B_CUDA_TRY(cudaFuncSetAttribute(score_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        const dim3 grid((unsigned)cdiv(nk, kTile), (unsigned)units);
+        score_kernel<D><<<grid, 128, smem, s>>>(qm, km, nq, nk, H, tiles, unit, score);
+    }
+    H3B_CUDA_TRY(cudaGetLastError());
+    return H3B_OK;
 }
 
 }  // namespace sel
@@ -185,8 +304,10 @@ extern "C" int h3b_block_means(const void* x, int64_t ld, int64_t hs, int64_t S,
     const unsigned grid = (unsigned)(cdiv(S, rows) * H);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const uint16_t* p = static_cast<const uint16_t*>(x);
-    if (D == 128) sel::means_kernel<128><<<grid, sel::kThreads, 0, s>>>(p, ld, hs, S, (int)H, (int)rows, out);
-    else sel::means_kernel<64><<<grid, sel::kThreads, 0, s>>>(p, ld, hs, S, (int)H, (int)rows, out);
+    if (D == 128 && rows == 128) sel::means_kernel<128, 128><<<grid, sel::kThreads, 0, s>>>(p, ld, hs, S, (int)H, out);
+    else if (D == 128) sel::means_kernel<128, 64><<<grid, sel::kThreads, 0, s>>>(p, ld, hs, S, (int)H, out);
+    else if (rows == 128) sel::means_kernel<64, 128><<<grid, sel::kThreads, 0, s>>>(p, ld, hs, S, (int)H, out);
+    else sel::means_kernel<64, 64><<<grid, sel::kThreads, 0, s>>>(p, ld, hs, S, (int)H, out);
     H3B_CUDA_TRY(cudaGetLastError());
     return H3B_OK;
 }
@@ -207,7 +328,8 @@ extern "C" int h3b_select_blocks(const float* qm, const float* km, int64_t nq, i
     H3B_REQUIRE(topk >= 0 && topk <= nk, "h3b_select_blocks: topk=%lld must lie in [0, %lld]", (long long)topk,
                 (long long)nk);
     if (nq == 0 || topk == 0) return H3B_OK;
-    H3B_REQUIRE(qm && km && blocks && workspace && aligned(workspace, 8), "h3b_select_blocks: NULL pointer");
+    H3B_REQUIRE(qm && km && blocks && workspace && aligned(workspace, 8) && aligned(qm, 16) && aligned(km, 16),
+                "h3b_select_blocks: NULL pointer, or means not 16-byte aligned");
     const int64_t unit = sel::kTile * nk * 8;
     const int tiles = (int)cdiv(nq, sel::kTile);
     const int64_t units = (int64_t)tiles * H;
@@ -218,11 +340,22 @@ extern "C" int h3b_select_blocks(const float* qm, const float* km, int64_t nq, i
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     for (int64_t u = 0; u < units; u += per) {
         const int64_t m = units - u < per ? units - u : per;
-        const dim3 grid((unsigned)cdiv(nk, sel::kTile), (unsigned)m);
         double* score = static_cast<double*>(workspace);
-        sel::score_kernel<<<grid, 256, 0, s>>>(qm, km, (int)nq, nk, (int)H, (int)D, tiles, u, score);
-        sel::topk_kernel<<<(unsigned)(m * sel::kTile), sel::kThreads, 0, s>>>(score, (int)nq, nk, tiles, u, (int)topk,
-                                                                             blocks);
+        if (int rc = D == 128 ? sel::scores<128>(qm, km, (int)nq, nk, (int)H, tiles, u, m, score, s)
+                              : sel::scores<64>(qm, km, (int)nq, nk, (int)H, tiles, u, m, score, s))
+            return rc;
+        const int held = (int)cdiv(nk, sel::kThreads), per = nq < sel::kTile ? (int)nq : sel::kTile;
+        const unsigned rows = (unsigned)(m * per);
+        if (held == 1)
+            sel::topk_kernel<1><<<rows, sel::kThreads, 0, s>>>(score, (int)nq, nk, tiles, u, (int)topk, per, blocks);
+        else if (held <= 4)
+            sel::topk_kernel<4><<<rows, sel::kThreads, 0, s>>>(score, (int)nq, nk, tiles, u, (int)topk, per, blocks);
+        else if (held <= 8)
+            sel::topk_kernel<8><<<rows, sel::kThreads, 0, s>>>(score, (int)nq, nk, tiles, u, (int)topk, per, blocks);
+        else if (held <= 16)
+            sel::topk_kernel<16><<<rows, sel::kThreads, 0, s>>>(score, (int)nq, nk, tiles, u, (int)topk, per, blocks);
+        else
+            sel::topk_kernel<0><<<rows, sel::kThreads, 0, s>>>(score, (int)nq, nk, tiles, u, (int)topk, per, blocks);
     }
     H3B_CUDA_TRY(cudaGetLastError());
     return H3B_OK;

@@ -61,6 +61,9 @@ SIGNATURES = [
     ("h3b_select_blocks", _I32, [_P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),
     ("h3b_block_sparse_attn", _I32, [_P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64,
                                      _F32, _P, _I64, _I64, _P, _I64, _P]),
+    ("h3b_sparse_attn_workspace", _I64, [_I64, _I64, _I64, _I64, _I64, _I32]),
+    ("h3b_sparse_attn", _I32, [_P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _F32, _P,
+                               _P, _I64, _I64, _P, _I64, _P]),
     ("h3b_a2a_inv_p2p", _I32, [_P, _I64, _PP, ctypes.POINTER(ctypes.c_int64), _I64, _I64, _I64, _I32, _P]),
 ]
 

@@ -20,7 +20,7 @@ import contextlib
 
 import torch
 
-from ._lib import check, lib, ptr, require_cuda, stream_of
+from ._lib import check, lib, require_cuda
 from .trace import span
 
 BF16 = torch.bfloat16
@@ -28,9 +28,17 @@ KEYS = 64    # tokens per scale of the cache, keys per sparse block
 QROWS = 128  # query rows that share a selection of key blocks
 
 
-def _on(t):
-    """Makes t's device the current one for the launches inside (nothing to do when it is)."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """Makes `device` the current one for the launches inside (nothing to do when it is)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _stream(device):
+    # (the handle alone: a torch.cuda.Stream object costs as much as the rest of a call's checks)
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _rows(name, t, like=None):
@@ -38,16 +46,19 @@ def _rows(name, t, like=None):
     if t.dtype != BF16 or t.dim() != 3:
         raise ValueError(f"{name} must be a bf16 [tokens, heads, head_dim] tensor, got {t.dtype} {tuple(t.shape)}")
     n, h, d = t.shape
-    if d not in (64, 128):
+    if d != 128 and d != 64:
         raise ValueError(f"{name}: head_dim {d} is not covered (64 or 128)")
     if h == 0:
         raise ValueError(f"{name}: no heads")
     if like is not None and (t.shape[1:] != like.shape[1:] or t.device != like.device):
         raise ValueError(f"{name} {tuple(t.shape)} on {t.device} does not go with {tuple(like.shape)} on {like.device}")
+    ld, hs, cs = t.stride()
     # the stride over a single token or head says nothing
-    ld = t.stride(0) if n > 1 else h * d
-    hs = t.stride(1) if h > 1 else d
-    if t.numel() and (t.stride(2) != 1 or ld % 8 or hs % 8 or ld <= 0 or hs <= 0 or t.data_ptr() % 16):
+    if n <= 1:
+        ld = h * d
+    if h == 1:
+        hs = d
+    if n and (cs != 1 or ld % 8 or hs % 8 or ld <= 0 or hs <= 0 or t.data_ptr() % 16):
         raise ValueError(f"{name}: strides {t.stride()} need a unit channel stride, positive token and head strides that "
                          "are multiples of 8 elements, and a 16-byte aligned start; pass a contiguous copy")
     return ld, hs
@@ -61,6 +72,10 @@ def _workspace(cache, q, segments):
     """(tensor or None, bytes): where the parts of a split over the keys meet and a cache's codes are widened."""
     n = lib.h3b_attn_workspace(cache, q.shape[0], q.shape[1], q.shape[2], segments)
     return (torch.empty(n, dtype=torch.uint8, device=q.device) if n else None), n
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 class KV8Cache:
@@ -83,17 +98,19 @@ class KV8Cache:
     @classmethod
     def wrap(cls, kq, vq, ks, vs, length):
         """A cache over existing codes and scales (contiguous, laid out as above), of which `length` tokens are held."""
-        if kq.dim() != 3 or kq.dtype != torch.int8 or kq.shape[0] == 0 or kq.shape[2] not in (64, 128) or kq.shape[1] % KEYS:
+        shape = kq.shape
+        if len(shape) != 3 or kq.dtype != torch.int8 or shape[0] == 0 or shape[2] not in (64, 128) or shape[1] % KEYS:
             raise ValueError("KV8Cache.wrap: kq must be int8 [heads, capacity, head_dim], capacity a multiple of "
-                             f"{KEYS} and head_dim 64 or 128; got {kq.dtype} {tuple(kq.shape)}")
-        scales = (kq.shape[0], kq.shape[1] // KEYS)
-        if vq.shape != kq.shape or vq.dtype != torch.int8 or any(
-                tuple(s.shape) != scales or s.dtype != torch.float32 for s in (ks, vs)):
+                             f"{KEYS} and head_dim 64 or 128; got {kq.dtype} {tuple(shape)}")
+        scales = (shape[0], shape[1] // KEYS)
+        if vq.shape != shape or vq.dtype != torch.int8 or ks.shape != scales or vs.shape != scales or \
+                ks.dtype != torch.float32 or vs.dtype != torch.float32:
             raise ValueError(f"KV8Cache.wrap: vq must match kq, ks and vs must be fp32 {scales}")
-        if not all(t.is_contiguous() and t.device == kq.device and t.data_ptr() % 16 == 0 for t in (kq, vq, ks, vs)):
-            raise ValueError("KV8Cache.wrap: codes and scales must be contiguous, 16-byte aligned and on one device")
-        if not 0 <= length <= kq.shape[1]:
-            raise ValueError(f"KV8Cache.wrap: length {length} outside the capacity {kq.shape[1]}")
+        for t in (kq, vq, ks, vs):
+            if not t.is_contiguous() or t.device != kq.device or t.data_ptr() % 16:
+                raise ValueError("KV8Cache.wrap: codes and scales must be contiguous, 16-byte aligned and on one device")
+        if not 0 <= length <= shape[1]:
+            raise ValueError(f"KV8Cache.wrap: length {length} outside the capacity {shape[1]}")
         self = cls.__new__(cls)
         self._take(kq, vq, ks, vs, int(length))
         return self
@@ -136,9 +153,9 @@ class KV8Cache:
                              f"within the capacity {self.capacity}")
         H, D = self.heads, self.head_dim
         if n:
-            with _on(k), span("kv8_write", 6 * n * H * D):
-                check(lib.h3b_kv8_write(ptr(k), kld, khs, ptr(v), vld, vhs, start, n, H, D, ptr(self.kq), ptr(self.vq),
-                                        ptr(self.ks), ptr(self.vs), self.capacity, stream_of(k)), "h3b_kv8_write")
+            with _on(k.device), span("kv8_write", 6 * n * H * D):
+                check(lib.h3b_kv8_write(_ptr(k), kld, khs, _ptr(v), vld, vhs, start, n, H, D, _ptr(self.kq), _ptr(self.vq),
+                                        _ptr(self.ks), _ptr(self.vs), self.capacity, _stream(k.device)), "h3b_kv8_write")
         self.length = start + n
         return self
 
@@ -154,9 +171,9 @@ class KV8Cache:
         n, H, D = stop - start, self.heads, self.head_dim
         k, v = (torch.empty((n, H, D), dtype=dtype, device=self.kq.device) for _ in "kv")
         if n:
-            with _on(k), span("kv8_read", 2 * n * H * D * (1 + k.element_size())):
-                check(lib.h3b_kv8_read(ptr(self.kq), ptr(self.vq), ptr(self.ks), ptr(self.vs), self.capacity, start, n,
-                                       H, D, ptr(k), ptr(v), int(dtype == torch.float32), stream_of(k)), "h3b_kv8_read")
+            with _on(k.device), span("kv8_read", 2 * n * H * D * (1 + k.element_size())):
+                check(lib.h3b_kv8_read(_ptr(self.kq), _ptr(self.vq), _ptr(self.ks), _ptr(self.vs), self.capacity, start, n,
+                                       H, D, _ptr(k), _ptr(v), int(dtype == torch.float32), _stream(k.device)), "h3b_kv8_read")
         return k, v
 
 
@@ -170,10 +187,10 @@ def kv8_attention(q, cache, scale=None):
     o = torch.empty((sq, H, D), dtype=BF16, device=q.device)
     if sq:
         ws, nbytes = _workspace(1, q, -(-cache.length // KEYS))
-        with _on(q), span("kv8_attn", 4.0 * sq * cache.length * H * D):
-            check(lib.h3b_kv8_attn(ptr(q), ld, hs, sq, H, D, ptr(cache.kq), ptr(cache.vq), ptr(cache.ks), ptr(cache.vs),
-                                   cache.capacity, cache.length, _scale(scale, D), ptr(o), H * D, D,
-                                   ptr(ws), nbytes, stream_of(q)), "h3b_kv8_attn")
+        with _on(q.device), span("kv8_attn", 4.0 * sq * cache.length * H * D):
+            check(lib.h3b_kv8_attn(_ptr(q), ld, hs, sq, H, D, _ptr(cache.kq), _ptr(cache.vq), _ptr(cache.ks), _ptr(cache.vs),
+                                   cache.capacity, cache.length, _scale(scale, D), _ptr(o), H * D, D,
+                                   _ptr(ws), nbytes, _stream(q.device)), "h3b_kv8_attn")
     return o
 
 
@@ -193,8 +210,8 @@ def block_means(x, rows=KEYS, out=None):
     elif tuple(out.shape) != shape or out.dtype != torch.float32 or not out.is_contiguous() or out.device != x.device:
         raise ValueError(f"block_means: out must be contiguous fp32 {shape} on {x.device}")
     if n:
-        with _on(x), span("block_means", 2 * x.numel()):
-            check(lib.h3b_block_means(ptr(x), ld, hs, n, H, D, rows, ptr(out), stream_of(x)), "h3b_block_means")
+        with _on(x.device), span("block_means", 2 * x.numel()):
+            check(lib.h3b_block_means(_ptr(x), ld, hs, n, H, D, rows, _ptr(out), _stream(x.device)), "h3b_block_means")
     return out
 
 
@@ -216,9 +233,9 @@ def select_blocks(qm, km, topk):
     blocks = torch.empty((H, nq, topk), dtype=torch.int32, device=qm.device)
     if nq and topk:
         ws = torch.empty(lib.h3b_select_blocks_workspace(nq, nk, H), dtype=torch.uint8, device=qm.device)
-        with _on(qm), span("select_blocks", 2.0 * nq * nk * H * D, launches=2):
-            check(lib.h3b_select_blocks(ptr(qm), ptr(km), nq, nk, H, D, topk, ptr(blocks), ptr(ws), ws.numel(),
-                                        stream_of(qm)), "h3b_select_blocks")
+        with _on(qm.device), span("select_blocks", 2.0 * nq * nk * H * D, launches=2):
+            check(lib.h3b_select_blocks(_ptr(qm), _ptr(km), nq, nk, H, D, topk, _ptr(blocks), _ptr(ws), ws.numel(),
+                                        _stream(qm.device)), "h3b_select_blocks")
     return blocks
 
 
@@ -241,21 +258,37 @@ def block_sparse_attention(q, k, v, blocks, scale=None):
     o = torch.empty((sq, H, D), dtype=BF16, device=q.device)
     if sq:
         ws, nbytes = _workspace(0, q, n)
-        with _on(q), span("sparse_attn", 4.0 * sq * n * KEYS * H * D):
-            check(lib.h3b_block_sparse_attn(ptr(q), qld, qhs, sq, H, D, ptr(k), kld, khs, ptr(v), vld, vhs, k.shape[0],
-                                            ptr(blocks), n, _scale(scale, D), ptr(o), H * D, D,
-                                            ptr(ws), nbytes, stream_of(q)), "h3b_block_sparse_attn")
+        with _on(q.device), span("sparse_attn", 4.0 * sq * n * KEYS * H * D):
+            check(lib.h3b_block_sparse_attn(_ptr(q), qld, qhs, sq, H, D, _ptr(k), kld, khs, _ptr(v), vld, vhs, k.shape[0],
+                                            _ptr(blocks), n, _scale(scale, D), _ptr(o), H * D, D,
+                                            _ptr(ws), nbytes, _stream(q.device)), "h3b_block_sparse_attn")
     return o
 
 
 def sparse_attention(q, k, v, topk, scale=None, k_means=None, return_blocks=False):
     """block_sparse_attention over the topk blocks of 64 keys that select_blocks finds for each block of 128 query
     rows.  k_means: block_means(k) if the program keeps it.  With return_blocks, (o, blocks)."""
-    require_cuda(q, k, v)
-    if k_means is None:
-        k_means = block_means(k, KEYS)
-    elif k_means.shape[0] != -(-k.shape[0] // KEYS):
-        raise ValueError(f"sparse_attention: k_means has {k_means.shape[0]} blocks for {k.shape[0]} keys")
-    blocks = select_blocks(block_means(q, QROWS), k_means, topk)
-    o = block_sparse_attention(q, k, v, blocks, scale)
+    require_cuda(q, k, v, k_means)
+    (qld, qhs), (kld, khs), (vld, vhs) = _rows("q", q), _rows("k", k, q), _rows("v", v, q)
+    (sq, H, D), sk = q.shape, k.shape[0]
+    nk = -(-sk // KEYS)
+    if v.shape[0] != sk:
+        raise ValueError(f"sparse_attention: {sk} keys and {v.shape[0]} values")
+    if topk < 0:
+        raise ValueError(f"sparse_attention: topk {topk}")
+    if k_means is not None and (k_means.shape != (nk, H, D) or k_means.dtype != torch.float32 or
+                                not k_means.is_contiguous() or k_means.device != q.device):
+        raise ValueError(f"sparse_attention: k_means must be contiguous fp32 {(nk, H, D)} on {q.device}, got "
+                         f"{k_means.dtype} {tuple(k_means.shape)}")
+    topk = min(int(topk), nk)
+    blocks = torch.empty((H, -(-sq // QROWS), topk), dtype=torch.int32, device=q.device)
+    o = torch.empty((sq, H, D), dtype=BF16, device=q.device)
+    if sq:
+        has = int(k_means is not None)
+        nbytes = lib.h3b_sparse_attn_workspace(sq, sk, H, D, topk, has)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        with _on(q.device), span("sparse_attn", 4.0 * sq * topk * KEYS * H * D, launches=5 - has):
+            check(lib.h3b_sparse_attn(_ptr(q), qld, qhs, sq, H, D, _ptr(k), kld, khs, _ptr(v), vld, vhs, sk, _ptr(k_means),
+                                      topk, _scale(scale, D), _ptr(blocks), _ptr(o), H * D, D, _ptr(ws), nbytes,
+                                      _stream(q.device)), "h3b_sparse_attn")
     return (o, blocks) if return_blocks else o

@@ -43,12 +43,16 @@ class Trace:
         return out
 
 
-@contextlib.contextmanager
+_OFF = contextlib.nullcontext()
+
+
 def span(name, work=0.0, launches=1):
-    t = _active
-    if t is None:
-        yield
-        return
+    """Context of one op: records it in the active Trace, does nothing without one."""
+    return _OFF if _active is None else _span(_active, name, work, launches)
+
+
+@contextlib.contextmanager
+def _span(t, name, work, launches):
     e0 = torch.cuda.Event(enable_timing=True)
     e1 = torch.cuda.Event(enable_timing=True)
     e0.record()

@@ -79,6 +79,23 @@ def test_attention_refusals():
     refused("h3b_block_sparse_attn", sparse(D=80), "head_dim")
 
 
+def test_sparse_attention_refusals():
+    def sparse(q=P16, Sq=200, Sk=100, H=2, D=128, topk=2, ws=P16, size=1 << 30, k=P16):
+        return lib.h3b_sparse_attn(q, 256, 128, Sq, H, D, k, 256, 128, P16, 256, 128, Sk, P0, topk, 1.0, P16, P16, 256, 128,
+                                   ws, size, P0)
+    refused("h3b_sparse_attn", sparse(D=32), "head_dim")
+    refused("h3b_sparse_attn", sparse(H=0), "heads")
+    refused("h3b_sparse_attn", sparse(Sq=-1), "rows")
+    refused("h3b_sparse_attn", sparse(topk=-1), "topk")
+    refused("h3b_sparse_attn", sparse(ws=P0), "workspace")
+    refused("h3b_sparse_attn", sparse(size=100), "workspace")
+    refused("h3b_block_means", sparse(k=P2), "aligned")
+    # query means, key means (unless kept) and the scores
+    assert lib.h3b_sparse_attn_workspace(200, 100, 2, 128, 2, 0) == 2048 + 2048 + 2 * 64 * 2 * 8
+    assert lib.h3b_sparse_attn_workspace(200, 100, 2, 128, 2, 1) == 2048 + 2 * 64 * 2 * 8
+    assert lib.h3b_sparse_attn_workspace(200, 100, 2, 96, 2, 1) == 0
+
+
 def test_selection_refusals():
     def means(D=128, rows=64, x=P16, ld=128):
         return lib.h3b_block_means(x, ld, 128, 5, 1, D, rows, P16, P0)
