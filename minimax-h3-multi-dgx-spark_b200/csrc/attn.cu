@@ -728,7 +728,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 // instructions for 8 rows, 40% of what an SM can issue in the time that HBM
 // takes to deliver them.
 
-constexpr int kRowWarps = 4;   // of a CTA, each with its own segments
+// Warps of a CTA, each with its own segments: 4, or 8 where that spares the split
+// of a short cache and the join (one row over 512 tokens).
+constexpr int kRowWarps = 4, kRowWarpsMost = 8;
 constexpr float kRowSlack = 4.0f, kRowBias = 11.0f;
 // Up to this many rows the rows kernel reads the codes once per 16 rows (from L2
 // after the first); beyond, they are widened once for the pair kernel.
@@ -762,16 +764,17 @@ __device__ __forceinline__ uint32_t half_codes(uint32_t x) {
 // two: 0.248 ms instead of 0.302 for a row over 131071 tokens of 40 heads).
 constexpr int row_ctas(int64_t D, int groups) { return groups == 2 ? 2 : D == 128 ? 3 : 4; }
 
-template <int D, int GROUPS>
-__global__ void __launch_bounds__(32 * kRowWarps, row_ctas(D, GROUPS)) rows_kernel(const __grid_constant__ Args a) {
+template <int D, int GROUPS, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, row_ctas(D, GROUPS) * kRowWarps / WARPS)
+    rows_kernel(const __grid_constant__ Args a) {
     constexpr int kRows = 8 * GROUPS;
     constexpr int kC = D / 4;     // channels of a thread's keys (scores)
     constexpr int kN = D / 8;     // channels of a thread's keys (output)
     constexpr int kKW = kC / 16;  // uint4 a key
     constexpr int kNW = kN / 4;   // words a key (output)
     using Piece = typename std::conditional<D == 128, uint4, uint2>::type;  // kN codes
-    __shared__ float so[kRowWarps][kRows][D];
-    __shared__ float sm[kRowWarps][kRows], sl[kRowWarps][kRows];
+    __shared__ float so[WARPS][kRows][D];
+    __shared__ float sm[WARPS][kRows], sl[WARPS][kRows];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     // row groups first: CTAs that run together share a head's codes in L2
     const uint32_t tiles = (uint32_t)((a.Sq + kRows - 1) / kRows);
@@ -779,6 +782,31 @@ __global__ void __launch_bounds__(32 * kRowWarps, row_ctas(D, GROUPS)) rows_kern
     const int64_t row0 = (int64_t)(blockIdx.x - rest * tiles) * kRows;
     const int part = (int)(rest / (uint32_t)a.H), h = (int)(rest - part * (uint32_t)a.H);
     const int rows = (int)min((int64_t)kRows, a.Sq - row0);
+
+    // this warp's segments: seg0, seg0 + WARPS, .. below seg1
+    const int64_t seg1 = a.segs * (part + 1) / a.parts, seg0 = a.segs * part / a.parts + warp;
+    const int8_t* kbase = a.codes[0] + ((int64_t)h * a.cap + g) * D + c * kC;
+    const int8_t* vbase = a.codes[1] + ((int64_t)h * a.cap + 2 * c) * D + g * kN;
+    const float* ks = a.scales[0] + (int64_t)h * (a.cap / kSeg);
+    const float* vs = a.scales[1] + (int64_t)h * (a.cap / kSeg);
+    uint4 kx[2][kKW];
+    Piece vx[4];
+    auto fetch = [&](int64_t seg, int turn) {
+        const int64_t at = (seg * kSeg + turn * 16) * D;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int w = 0; w < kKW; ++w) kx[t][w] = __ldcs(reinterpret_cast<const uint4*>(kbase + at + t * 8 * D) + w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            vx[k] = __ldcs(reinterpret_cast<const Piece*>(vbase + at + ((k & 1) + (k & 2) * 4) * D));
+    };
+    float sk = 0.0f, sv = 0.0f;
+    if (seg0 < seg1) {
+        fetch(seg0, 0);
+        sk = __ldg(ks + seg0);
+        sv = __ldg(vs + seg0);
+    }
 
     // Q^T: row g of each group, channels kC c ..
     uint32_t q[GROUPS][kC / 2];
@@ -823,37 +851,13 @@ __global__ void __launch_bounds__(32 * kRowWarps, row_ctas(D, GROUPS)) rows_kern
         l[r][0] = l[r][1] = 0.0f;
     }
 
-    // this warp's segments: seg0, seg0 + kRowWarps, .. below seg1
-    const int64_t seg1 = a.segs * (part + 1) / a.parts, seg0 = a.segs * part / a.parts + warp;
-    const int8_t* kbase = a.codes[0] + ((int64_t)h * a.cap + g) * D + c * kC;
-    const int8_t* vbase = a.codes[1] + ((int64_t)h * a.cap + 2 * c) * D + g * kN;
-    const float* ks = a.scales[0] + (int64_t)h * (a.cap / kSeg);
-    const float* vs = a.scales[1] + (int64_t)h * (a.cap / kSeg);
-    uint4 kx[2][kKW];
-    Piece vx[4];
-    auto fetch = [&](int64_t seg, int turn) {
-        const int64_t at = (seg * kSeg + turn * 16) * D;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int w = 0; w < kKW; ++w) kx[t][w] = __ldcs(reinterpret_cast<const uint4*>(kbase + at + t * 8 * D) + w);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            vx[k] = __ldcs(reinterpret_cast<const Piece*>(vbase + at + ((k & 1) + (k & 2) * 4) * D));
-    };
-    float sk = 0.0f, sv = 0.0f;
-    if (seg0 < seg1) {
-        fetch(seg0, 0);
-        sk = __ldg(ks + seg0);
-        sv = __ldg(vs + seg0);
-    }
-    for (int64_t seg = seg0; seg < seg1; seg += kRowWarps) {
+    for (int64_t seg = seg0; seg < seg1; seg += WARPS) {
         const float fk = sk, fv = sv;
         const int valid = (int)min((int64_t)kSeg, a.keys - seg * kSeg);
-        const bool more = seg + kRowWarps < seg1;
+        const bool more = seg + WARPS < seg1;
         if (more) {
-            sk = __ldg(ks + seg + kRowWarps);
-            sv = __ldg(vs + seg + kRowWarps);
+            sk = __ldg(ks + seg + WARPS);
+            sv = __ldg(vs + seg + WARPS);
         }
         float os[GROUPS][kN / 2][4];  // this block's output, without its scale
 #pragma unroll
@@ -874,7 +878,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, row_ctas(D, GROUPS)) rows_kern
 #pragma unroll
                 for (int w = 0; w < kNW; ++w) vc[k][w] = reinterpret_cast<const uint32_t*>(&vx[k])[w] ^ 0x80808080u;
             if (turn + 1 < kSeg / 16) fetch(seg, turn + 1);
-            else if (more) fetch(seg + kRowWarps, 0);
+            else if (more) fetch(seg + WARPS, 0);
             float s[GROUPS][4];
 #pragma unroll
             for (int r = 0; r < GROUPS; ++r) s[r][0] = s[r][1] = s[r][2] = s[r][3] = 0.0f;
@@ -970,15 +974,15 @@ __global__ void __launch_bounds__(32 * kRowWarps, row_ctas(D, GROUPS)) rows_kern
             }
         }
     __syncthreads();
-    for (int e = threadIdx.x; e < rows * (D / 2); e += 32 * kRowWarps) {
+    for (int e = threadIdx.x; e < rows * (D / 2); e += 32 * WARPS) {
         const int r = e / (D / 2), ch = 2 * (e % (D / 2));
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm[w][r]);
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, sm[w][r]);
         const float ref = top == -INFINITY ? 0.0f : top;
         float total = 0.0f, x = 0.0f, y = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             const float f = ex2(sm[w][r] - ref);
             total += f * sl[w][r];
             x += f * so[w][r][ch];
@@ -1119,6 +1123,7 @@ static int64_t row_parts_of(int64_t tiles, int64_t segs, int ctas) {
 
 struct Plan {
     bool rows;               // the rows kernel
+    int warps;               // of its CTAs
     int64_t heads;           // heads a launch (and of the widened copy)
     int64_t parts;           // of the keys
     int64_t join_at, bytes;  // in the workspace
@@ -1127,12 +1132,14 @@ struct Plan {
 constexpr int64_t kWideBytes = 256ll << 20;  // of widened heads at a time (one head at least)
 
 static Plan plan(bool cache, int64_t Sq, int64_t H, int64_t D, int64_t segs) {
-    Plan p{false, H, 1, 0, 0};
+    Plan p{false, 0, H, 1, 0, 0};
     if (segs == 0) return p;
     if (cache && Sq <= kRowsMost) {
         p.rows = true;
         const int groups = Sq <= 8 ? 1 : 2;
         p.parts = row_parts_of(cdiv(Sq, 8 * groups) * H, segs, row_ctas(D, groups));
+        p.warps = groups == 1 && p.parts <= 2 && segs > kRowWarps && H <= sm_count() ? kRowWarpsMost : kRowWarps;
+        if (p.warps == kRowWarpsMost) p.parts = 1;
         p.bytes = p.parts > 1 ? p.parts * H * Sq * (D + 2) * 4 : 0;
         return p;
     }
@@ -1171,8 +1178,9 @@ static int launch_all(Args& a, bool cache, const Plan& p, char* ws, cudaStream_t
     a.parts = (int)p.parts;
     a.heads = a.H;
     if (p.rows) {
-        if (a.Sq <= 8) rows_kernel<D, 1><<<(unsigned)(a.H * p.parts), 32 * kRowWarps, 0, s>>>(a);
-        else rows_kernel<D, 2><<<(unsigned)(cdiv(a.Sq, 16) * a.H * p.parts), 32 * kRowWarps, 0, s>>>(a);
+        if (p.warps == kRowWarpsMost) rows_kernel<D, 1, kRowWarpsMost><<<(unsigned)a.H, 32 * kRowWarpsMost, 0, s>>>(a);
+        else if (a.Sq <= 8) rows_kernel<D, 1, kRowWarps><<<(unsigned)(a.H * p.parts), 32 * kRowWarps, 0, s>>>(a);
+        else rows_kernel<D, 2, kRowWarps><<<(unsigned)(cdiv(a.Sq, 16) * a.H * p.parts), 32 * kRowWarps, 0, s>>>(a);
         if (p.parts > 1) join_kernel<D><<<(unsigned)(a.Sq * a.H), 128, 0, s>>>(a);
         H3B_CUDA_TRY(cudaGetLastError());
         return H3B_OK;

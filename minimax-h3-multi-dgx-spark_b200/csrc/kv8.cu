@@ -19,6 +19,7 @@ namespace kv8 {
 
 constexpr int kBlock = 64;  // tokens per scale
 constexpr int kThreads = 256;
+constexpr int kWriteThreads = 128;
 
 struct WriteArgs {
     const uint16_t* x[2];  // k, v: [n, H, D], strides in elements
@@ -35,41 +36,45 @@ __device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
 
 // One CTA per block of 64 tokens and head (blockIdx.x) and per K / V
 // (blockIdx.y).  A thread holds 8 consecutive channels of PASSES tokens in
-// registers between the maximum and the division, so x is read once.
+// registers between the maximum and the division, so x is read once.  Bound by
+// HBM in principle (x once, codes once); 128 threads with twice the tokens each
+// rather than 256, because what a thread does besides its tokens counts here.
 template <int D>
-__global__ void __launch_bounds__(kThreads) write_kernel(WriteArgs a) {
-    constexpr int kCols = D / 8;              // threads along the channels
-    constexpr int kRows = kThreads / kCols;   // tokens per pass
+__global__ void __launch_bounds__(kWriteThreads) write_kernel(const __grid_constant__ WriteArgs a) {
+    constexpr int kCols = D / 8;                  // threads along the channels
+    constexpr int kRows = kWriteThreads / kCols;  // tokens per pass
     constexpr int kPasses = kBlock / kRows;
     const int which = blockIdx.y;
-    const int h = (int)(blockIdx.x % (unsigned)a.H);
-    const int64_t b = a.start / kBlock + blockIdx.x / (unsigned)a.H;
-    const int64_t end = a.start + a.n;
+    const unsigned nth = blockIdx.x / (unsigned)a.H;
+    const int h = (int)(blockIdx.x - nth * (unsigned)a.H);
+    const int64_t b = a.start / kBlock + nth;
+    // new tokens are rows first .. last - 1 of the block, older ones lie before
+    const int first = (int)max(a.start - b * kBlock, (int64_t)0);
+    const int last = (int)min(a.start + a.n - b * kBlock, (int64_t)kBlock);
     const int col = threadIdx.x % kCols, row = threadIdx.x / kCols;
-    int8_t* codes = a.codes[which] + ((int64_t)h * a.cap + b * kBlock) * D + col * 8;
+    int8_t* codes = a.codes[which] + ((int64_t)h * a.cap + b * kBlock + row) * D + col * 8;
     float* scale = a.scales[which] + (int64_t)h * (a.cap / kBlock) + b;
+    const int64_t ld = a.ld[which];
+    const uint16_t* x = a.x[which] + (b * kBlock - a.start + row) * ld + h * a.hs[which] + col * 8;
 
     uint4 v[kPasses];
     uint32_t pair = 0;  // maxima of the low and of the high halves' bits
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
-        const int64_t t = b * kBlock + row + p * kRows;
+        const int r = row + p * kRows;
         v[p] = make_uint4(0, 0, 0, 0);
-        if (t >= a.start && t < end)
-            v[p] = *reinterpret_cast<const uint4*>(a.x[which] + (t - a.start) * a.ld[which] + h * a.hs[which] + col * 8);
+        if (r >= first && r < last) v[p] = __ldcs(reinterpret_cast<const uint4*>(x + p * kRows * ld));
     }
+    const bool stays = first > 0;  // older tokens in this block
+    const float older = stays ? *scale : 0.0f;
 #pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-        pair = absmax_bits8(v[p], pair);
-    }
-    __shared__ uint32_t tops[kThreads / 32];
+    for (int p = 0; p < kPasses; ++p) pair = absmax_bits8(v[p], pair);
+    __shared__ uint32_t tops[kWriteThreads / 32];
     uint32_t top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(fold_absmax_bits(pair)));
     if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
-    const bool stays = a.start > b * kBlock;  // older tokens in this block
-    const float older = stays ? *scale : 0.0f;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) top = max(top, tops[w]);
+    for (int w = 0; w < kWriteThreads / 32; ++w) top = max(top, tops[w]);
     // a NaN's quotient is a NaN: the order of the bit patterns still holds below
     float s = __fdiv_rn(__uint_as_float(top), 127.0f);
     if ((__float_as_uint(older) & 0x7FFFFFFFu) > (__float_as_uint(s) & 0x7FFFFFFFu)) s = older;
@@ -80,15 +85,13 @@ __global__ void __launch_bounds__(kThreads) write_kernel(WriteArgs a) {
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
         const int r = row + p * kRows;
-        const int64_t t = b * kBlock + r;
-        if (t >= end) continue;
-        uint2* dst = reinterpret_cast<uint2*>(codes + (int64_t)r * D);
-        if (t >= a.start) {
-            float x[8];
-            unpack8(v[p], x);
+        uint2* dst = reinterpret_cast<uint2*>(codes + p * kRows * D);
+        if (r >= first && r < last) {
+            float f[8];
+            unpack8(v[p], f);
             // (the scale is the block's absmax / 127 or larger, so no code leaves [-127, 127])
-            *dst = live ? quant8(x, s, inverse) : make_uint2(0u, 0u);
-        } else if (grew) {
+            *dst = live ? quant8(f, s, inverse) : make_uint2(0u, 0u);
+        } else if (grew && r < first) {
             const uint2 old = *dst;
             int c[8];
 #pragma unroll
@@ -113,7 +116,7 @@ struct ReadArgs {
 
 // One CTA per block of 64 tokens and head, per K / V; 8 codes a thread and pass.
 template <int D, bool F32>
-__global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
+__global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ ReadArgs a) {
     constexpr int kCols = D / 8;
     constexpr int kRows = kThreads / kCols;
     const int which = blockIdx.y;
@@ -184,8 +187,8 @@ extern "C" int h3b_kv8_write(const void* k, int64_t k_ld, int64_t k_hs, const vo
     const int64_t blocks = cdiv(start + n, kv8::kBlock) - start / kv8::kBlock;
     const dim3 grid((unsigned)(blocks * H), 2);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (D == 128) kv8::write_kernel<128><<<grid, kv8::kThreads, 0, s>>>(a);
-    else kv8::write_kernel<64><<<grid, kv8::kThreads, 0, s>>>(a);
+    if (D == 128) kv8::write_kernel<128><<<grid, kv8::kWriteThreads, 0, s>>>(a);
+    else kv8::write_kernel<64><<<grid, kv8::kWriteThreads, 0, s>>>(a);
     H3B_CUDA_TRY(cudaGetLastError());
     return H3B_OK;
 }

@@ -153,15 +153,15 @@ __device__ __forceinline__ uint64_t sort_key(double s) {
 
 // One CTA per (head, query block): radix selection of the topk-th largest key,
 // eight bits a pass until all keys that share the digits so far are taken, then
-// the chosen indices in ascending order.  A thread has consecutive keys: HELD of
-// them in registers, or as many as it takes, read again every pass (HELD 0).
+// the chosen indices in ascending order.  HELD keys a thread (every kThreads-th)
+// stay in registers; with HELD 0 all are read again every pass.
 template <int HELD>
-__global__ void __launch_bounds__(kThreads) topk_kernel(const double* __restrict__ score, int nq, int64_t nk, int tiles,
+__global__ void __launch_bounds__(kThreads, HELD <= 8 ? 6 : 4) topk_kernel(const double* __restrict__ score, int nq, int64_t nk, int tiles,
                                                         int64_t unit0, int topk, int per, int32_t* __restrict__ blocks) {
     constexpr int kWarps = kThreads / 32;
     __shared__ int hist[256];
     __shared__ int s_digit, s_left, s_count;
-    __shared__ int warp_n[kWarps][2];
+    __shared__ int taken[2][(HELD > 0 ? HELD : 1) * kWarps];  // above the prefix, with it: by round and warp
     const int64_t unit = unit0 + blockIdx.x / per;
     const int h = (int)(unit / tiles), r = blockIdx.x % per;  // `per` rows of a unit are in the launch
     const int64_t i = (unit % tiles) * kTile + r;
@@ -173,19 +173,24 @@ __global__ void __launch_bounds__(kThreads) topk_kernel(const double* __restrict
         for (int64_t j = threadIdx.x; j < nk; j += kThreads) out[j] = (int32_t)j;
         return;
     }
-    const int mine = HELD > 0 ? HELD : (int)((nk + kThreads - 1) / kThreads);
-    const int64_t j0 = (int64_t)threadIdx.x * mine;
+    const int rounds = (int)((nk + kThreads - 1) / kThreads);
     uint64_t held[HELD > 0 ? HELD : 1];
     if constexpr (HELD > 0) {
 #pragma unroll
-        for (int t = 0; t < HELD; ++t) held[t] = j0 + t < nk ? sort_key(row[j0 + t]) : 0;
+        for (int t = 0; t < HELD; ++t) {
+            const int64_t j = threadIdx.x + t * kThreads;
+            held[t] = j < nk ? sort_key(row[j]) : 0;
+        }
     }
     auto each = [&](auto&& f) {
         if constexpr (HELD > 0) {
 #pragma unroll
-            for (int t = 0; t < HELD; ++t) f(j0 + t, held[t]);
+            for (int t = 0; t < HELD; ++t) f(threadIdx.x + t * kThreads, held[t], t);
         } else {
-            for (int t = 0; t < mine; ++t) f(j0 + t, j0 + t < nk ? sort_key(row[j0 + t]) : 0);
+            for (int t = 0; t < rounds; ++t) {
+                const int64_t j = threadIdx.x + (int64_t)t * kThreads;
+                f(j, j < nk ? sort_key(row[j]) : 0, t);
+            }
         }
     };
     uint64_t prefix = 0;
@@ -194,12 +199,16 @@ __global__ void __launch_bounds__(kThreads) topk_kernel(const double* __restrict
     for (;; shift -= 8) {
         hist[threadIdx.x] = 0;
         __syncthreads();
-        each([&](int64_t j, uint64_t key) {
-            // many keys share their leading digits: one addition for a warp's equal ones
+        each([&](int64_t j, uint64_t key, int) {
             const bool in = j < nk && (shift == 56 || (key >> (shift + 8)) == (prefix >> (shift + 8)));
             const uint32_t digit = in ? (uint32_t)(key >> shift) & 255u : 256u;
-            const uint32_t same = __match_any_sync(0xFFFFFFFFu, digit);
-            if (in && lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
+            if (shift >= 48) {
+                // most keys share their exponent's digits: one addition for a warp's equal ones
+                const uint32_t same = __match_any_sync(0xFFFFFFFFu, digit);
+                if (in && lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
+            } else if (in) {
+                atomicAdd(&hist[digit], 1);
+            }
         });
         __syncthreads();
         if (warp == 0) {
@@ -235,39 +244,79 @@ __global__ void __launch_bounds__(kThreads) topk_kernel(const double* __restrict
         if (all || shift == 0) break;
     }
     // every key above the prefix is taken, and the first `want` that have it
-    int gt = 0, eq = 0;
-    each([&](int64_t j, uint64_t key) {
-        const uint64_t head = key >> shift;
-        gt += j < nk && head > (prefix >> shift);
-        eq += j < nk && head == (prefix >> shift);
-    });
-    int g = gt, q = eq;  // scanned over the threads before
+    const uint32_t below = (1u << lane) - 1u;
+    const uint64_t bar = prefix >> shift;
+    if constexpr (HELD > 0) {
+        // counts of every round and warp, their sum before each, then the places
+        each([&](int64_t j, uint64_t key, int t) {
+            const uint64_t head = key >> shift;
+            const uint32_t mg = __ballot_sync(0xFFFFFFFFu, j < nk && head > bar),
+                           me = __ballot_sync(0xFFFFFFFFu, j < nk && head == bar);
+            if (lane == 0) {
+                taken[0][t * kWarps + warp] = __popc(mg);
+                taken[1][t * kWarps + warp] = __popc(me);
+            }
+        });
+        __syncthreads();
+        if (warp < 2) {
+            constexpr int kEach = (HELD * kWarps + 31) / 32;
+            int n[kEach], sum = 0;
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const int x = __shfl_up_sync(0xFFFFFFFFu, g, off), y = __shfl_up_sync(0xFFFFFFFFu, q, off);
-        if (lane >= off) g += x, q += y;
-    }
-    if (lane == 31) {
-        warp_n[warp][0] = g;
-        warp_n[warp][1] = q;
-    }
-    __syncthreads();
-    g -= gt;
-    q -= eq;
+            for (int e = 0; e < kEach; ++e) {
+                const int at = lane * kEach + e;
+                n[e] = at < HELD * kWarps ? taken[warp][at] : 0;
+                sum += n[e];
+            }
+            int before = sum;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w)
-        if (w < warp) {
-            g += warp_n[w][0];
-            q += warp_n[w][1];
+            for (int off = 1; off < 32; off <<= 1) {
+                const int y = __shfl_up_sync(0xFFFFFFFFu, before, off);
+                if (lane >= off) before += y;
+            }
+            before -= sum;
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const int at = lane * kEach + e;
+                if (at < HELD * kWarps) taken[warp][at] = before;
+                before += n[e];
+            }
         }
-    each([&](int64_t j, uint64_t key) {
-        const uint64_t head = key >> shift;
-        if (j >= nk || head < (prefix >> shift)) return;
-        const bool equal = head == (prefix >> shift);
-        if (!equal || q < want) out[g + min(q, want)] = (int32_t)j;
-        g += !equal;
-        q += equal;
-    });
+        __syncthreads();
+        each([&](int64_t j, uint64_t key, int t) {
+            const uint64_t head = key >> shift;
+            const bool gt = j < nk && head > bar, eq = j < nk && head == bar;
+            const uint32_t mg = __ballot_sync(0xFFFFFFFFu, gt), me = __ballot_sync(0xFFFFFFFFu, eq);
+            const int g = taken[0][t * kWarps + warp] + __popc(mg & below), q = taken[1][t * kWarps + warp] + __popc(me & below);
+            if (gt || (eq && q < want)) out[g + min(q, want)] = (int32_t)j;
+        });
+    } else {
+        int above = 0, equal = 0;  // so far, before this round's
+        each([&](int64_t j, uint64_t key, int) {
+            const uint64_t head = key >> shift;
+            const bool gt = j < nk && head > bar, eq = j < nk && head == bar;
+            const uint32_t mg = __ballot_sync(0xFFFFFFFFu, gt), me = __ballot_sync(0xFFFFFFFFu, eq);
+            if (lane == 0) {
+                taken[0][warp] = __popc(mg);
+                taken[1][warp] = __popc(me);
+            }
+            __syncthreads();
+            int g = above, q = equal;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                if (w < warp) {
+                    g += taken[0][w];
+                    q += taken[1][w];
+                }
+                above += taken[0][w];
+                equal += taken[1][w];
+            }
+            g += __popc(mg & below);
+            q += __popc(me & below);
+            if (gt || (eq && q < want)) out[g + min(q, want)] = (int32_t)j;
+            __syncthreads();
+        });
+    }
 }
 
 template <int D>
