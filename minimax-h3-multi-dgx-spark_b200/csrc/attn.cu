@@ -401,9 +401,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
     uint64_t *kv_full = bars, *kv_empty = bars + 4,  // of the groups
         *s_full = bars + 8, *p_full = bars + 12,     // [tile][buffer]
-        *q_full = bars + 16, *q_empty = bars + 18, *pv_done = bars + 20, *out_full = bars + 22, *drain = bars + 24,  // [tile]
-        *out_free = bars + 26;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 27);
+        *q_full = bars + 16, *q_empty = bars + 18, *pv_done = bars + 20, *o_full = bars + 22, *out_full = bars + 24,  // [tile]
+        *drain = bars + 26, *out_free = bars + 28;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -423,6 +423,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             mbar_init(q_full + t, 1);
             mbar_init(q_empty + t, 1);
             mbar_init(pv_done + t, 1);
+            mbar_init(o_full + t, 1);
             mbar_init(out_full + t, 4);
             mbar_init(drain + t, 1);
         }
@@ -456,10 +457,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             uint32_t g = 0;                    // groups so far
             uint32_t nq = 0, ns = 0, np = 0;   // this tile's items, scores and products so far
             auto wait = [&](uint64_t* bar, uint32_t phase) { ok = ok && await(bar, phase, abort_flag, a.status); };
-            // The products that group g is for: O += P V of step g - 2 (if the tile has that step; `fresh`: its item's
-            // first) and S = Q K^T of step g (the same; begin, end: its item's first and last).  S goes where P of
+            // The products that group g is for: O += P V of step g - 2 (if the tile has that step; fresh, final: its
+            // item's first and last) and S = Q K^T of step g (the same; begin, end).  S goes where P of
             // two steps before was, which the product before has read (MMAs run in order)
-            auto group = [&](bool output, bool fresh, bool scores, bool begin, bool end) {
+            auto group = [&](bool output, bool fresh, bool final, bool scores, bool begin, bool end) {
                 const uint32_t place = SRC == kWide ? g & 3u : 2 * t + (g & 1u);
                 const uint32_t off = place * (L::kGroup >> 4);
                 const uint32_t kv_phase = (SRC == kWide ? g >> 2 : g >> 1) & 1u, p_phase = (np >> 1) & 1u;
@@ -477,6 +478,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                     for (int j = 0; j < kSeg / 16; ++j)
                         mma_ts(tO, tS + 64 * buf + 8 * j, v0 + off + j * (2048 >> 4), id_o, j > 0 || !fresh);
                     umma_commit(pv_done + t);
+                    if (final) umma_commit(o_full + t);
                     ++np;
                 }
                 if (scores) {
@@ -497,23 +499,25 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 if (ok) umma_commit(kv_empty + place);
                 ++g;
             };
-            // steps two and one before: does the tile have them, and are they their items' first?
-            bool has2 = false, has1 = false, first2 = false, first1 = false;
+            // steps two and one before: does the tile have them, are they their items' first or last?
+            bool has2 = false, has1 = false, first2 = false, first1 = false, last2 = false, last1 = false;
             for (uint32_t item = blockIdx.x; ok && item < a.items; item += gridDim.x) {
                 const Item it = item_of<SRC>(a, item);
                 const bool has = t == 0 || it.both;
                 if (SRC == kBlocks && !has) continue;  // (there are no loads for it)
                 for (int i = 0; ok && i < it.steps; ++i) {
-                    group(has2, first2, has, i == 0, i + 1 == it.steps);
+                    group(has2, first2, last2, has, i == 0, i + 1 == it.steps);
                     has2 = has1;
                     first2 = first1;
+                    last2 = last1;
                     has1 = has;
                     first1 = i == 0;
+                    last1 = i + 1 == it.steps;
                 }
             }
             if (ok && g > 0) {
-                group(has2, first2, false, false, false);
-                if (ok) group(has1, first1, false, false, false);
+                group(has2, first2, last2, false, false, false);
+                if (ok) group(has1, first1, last1, false, false, false);
             }
             if (!ok) {
                 // no MMA of this thread stays in flight
@@ -627,6 +631,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 if (!(ok = wait(s_full + buf, step >> 1))) break;
                 tc_fence_after();
                 const uint32_t tX = tS + 64 * (step & 1u);
+                // (a wait cannot tell a phase from the second next: all products but the last are known to be done when
+                // S is there, and the next waits for this step's P)
                 auto product_done = [&] { ok = wait(pv_done + t, step - 1); };
                 const float sk = SRC == kBlocks ? scale2 : scale2 * f.sk;
                 if (f.n == kSeg)
@@ -638,10 +644,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full + buf);
             }
-            // one after the other: a wait tells a phase from the one before it only, and the last S came when all but
-            // the last two products were done
-            if (ok && step > 1) ok = wait(pv_done + t, step - 2);
-            if (!ok || !(ok = wait(pv_done + t, step - 1))) break;
+            if (!ok || !(ok = wait(o_full + t, outs))) break;
             tc_fence_after();
             const int64_t row = (int64_t)u.qt * kQRows + trow;
             const bool split = a.parts > 1;
