@@ -35,6 +35,7 @@ struct Args {
     int64_t segs;   // segments of 64 keys
     uint32_t items;  // pairs of tiles of the launch
     int heads, parts;  // heads of the launch, parts of the keys
+    bool turns;        // the exponentials of a pair's tiles take turns
     // parts of a split: O [parts, H, Sq, D], (reference maximum, sum) [parts, H, Sq, 2], H of the launch
     float* part_o;
     float* part_ml;
@@ -71,7 +72,7 @@ struct Smem {
     // K and V arrive in groups: the keys of a step with the values of the step two before it
     static constexpr int kGroup = 2 * kSegTile, kGroups = 4;
     static constexpr int kQ = 0, kKV = 2 * kTile, kO = kKV + kGroups * kGroup, kBars = kO + kTile;
-    static constexpr int kBytes = kBars + 256;
+    static constexpr int kBytes = kBars + 512;
 };
 
 // kind::f16 instruction descriptor: D fp32 (bits 4-5 = 1), A and B bf16 (7-9 = 1,
@@ -258,6 +259,27 @@ __device__ __forceinline__ bool await(uint64_t* bar, uint32_t phase, volatile in
     }
 }
 
+// The exponentials of the two tiles take turns: a warp of tile 0 and the one of
+// tile 1 that shares its scheduler, and so its special-function unit.  Left to
+// themselves the tiles fall into step, whatever distance they start with: both
+// compute exponentials at half the rate, and meanwhile nothing else (64 steps:
+// 987 TFLOP/s, with turns 1078).
+struct Turn {
+    uint64_t *mine, *other;  // null: the other tile is not there
+    uint32_t phase;
+    volatile int* abort_flag;
+    int* status;
+    __device__ __forceinline__ bool look() const { return !mine || mbar_try_wait(mine, phase & 1u); }
+    __device__ __forceinline__ void take(bool seen) const {
+        if (!__all_sync(0xFFFFFFFFu, seen)) await(mine, phase, abort_flag, status);  // (if it gives up, so will the next wait)
+        __syncwarp();
+    }
+    __device__ __forceinline__ void pass() const {
+        if (mine && (threadIdx.x & 31) == 0) mbar_arrive(other);
+    }
+};
+constexpr int kPassOn = 1;  // half of a step's exponentials before which the turn passes on (2: behind them)
+
 // One step of a row: S (64 columns at tS) -> P (bf16, 32 columns at tS), with the
 // running maximum and sum.  n: valid keys; sk, sv: factors of the scores (softmax
 // scale, log2 e and, for codes, the block's scale) and of the values.  TAIL: not
@@ -265,12 +287,13 @@ __device__ __forceinline__ bool await(uint64_t* bar, uint32_t phase, volatile in
 // may be rescaled; first: there is none.
 template <int D, Source SRC, bool TAIL, typename Wait>
 __device__ __forceinline__ void softmax_step(Row& st, uint32_t tS, uint32_t tO, bool first, int n, float sk, float sv,
-                                             const Wait& product_done) {
+                                             const Wait& product_done, const Turn& turn) {
     uint32_t r[2][32];
     tmem_ld32_async(tS, r[0]);
     tmem_ld32_async(tS + 32, r[1]);
     tmem_ready(r[0]);
     tmem_ready(r[1]);
+    const bool seen = turn.look();  // (asked here, answered below)
     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
     for (int e = 0; e < 64; e += 2) {
@@ -306,8 +329,10 @@ __device__ __forceinline__ void softmax_step(Row& st, uint32_t tS, uint32_t tO, 
     if (!(top < INFINITY)) st.l = __int_as_float(0x7FC00000);
     const float ref = st.m == -INFINITY ? 0.0f : st.m;
     float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+    turn.take(seen);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
+        if (c == kPassOn) turn.pass();
         uint32_t p[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -326,6 +351,7 @@ __device__ __forceinline__ void softmax_step(Row& st, uint32_t tS, uint32_t tO, 
         }
         tmem_st16(tS + c * 16, p);
     }
+    if (kPassOn == 2) turn.pass();
     sum[0] = add2(sum[0], sum[1]);
     st.l += sum[0].x + sum[0].y;
 }
@@ -402,8 +428,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     uint64_t *kv_full = bars, *kv_empty = bars + 4,  // of the groups
         *s_full = bars + 8, *p_full = bars + 12,     // [tile][buffer]
         *q_full = bars + 16, *q_empty = bars + 18, *pv_done = bars + 20, *o_full = bars + 22, *out_full = bars + 24,  // [tile]
-        *drain = bars + 26, *out_free = bars + 28;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
+        *drain = bars + 26, *out_free = bars + 28, *take = bars + 29;  // [tile][scheduler]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 37);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -428,6 +454,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             mbar_init(drain + t, 1);
         }
         mbar_init(out_free, 1);
+        for (int j = 0; j < 8; ++j) mbar_init(take + j, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -597,8 +624,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const uint32_t at = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + at + 128 * t, tO = tmem + at + 256 + 128 * t;
         const float scale2 = fabsf(a.scale) * kLog2e;
-        // this tile's steps and outputs so far, and the uses of the output's place by both tiles
-        uint32_t step = 0, outs = 0, turn = 0;
+        // this tile's steps and outputs so far, the uses of the output's place by both tiles, the steps of both
+        uint32_t step = 0, outs = 0, turn = 0, shared = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t phase) {
             return __all_sync(0xFFFFFFFFu, await(bar, phase, abort_flag, a.status)) != 0;
@@ -624,8 +651,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 return Factors{g.n, __ldg(a.scales[0] + b), __ldg(a.scales[1] + b)};
             };
             Factors ahead = factors(0);
+            const bool paired = it.both && a.turns;
             for (int i = 0; ok && i < it.steps; ++i, ++step) {
                 const Factors f = ahead;
+                // tile 1 follows tile 0's exponentials of the same step, tile 0 tile 1's of the step before
+                const Turn turns{paired ? take + (warp & 3) + 4 * t : nullptr, take + (warp & 3) + 4 * (1 - t),
+                                 shared + t - 1u, abort_flag, a.status};
+                if (paired) ++shared;
                 if (i + 1 < it.steps) ahead = factors(i + 1);
                 const int buf = 2 * t + (int)(step & 1u);
                 if (!(ok = wait(s_full + buf, step >> 1))) break;
@@ -636,9 +668,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 auto product_done = [&] { ok = wait(pv_done + t, step - 1); };
                 const float sk = SRC == kBlocks ? scale2 : scale2 * f.sk;
                 if (f.n == kSeg)
-                    softmax_step<D, SRC, false>(st, tX, tO, i == 0, f.n, sk, f.sv, product_done);
+                    softmax_step<D, SRC, false>(st, tX, tO, i == 0, f.n, sk, f.sv, product_done, turns);
                 else
-                    softmax_step<D, SRC, true>(st, tX, tO, i == 0, max(f.n, 0), sk, f.sv, product_done);
+                    softmax_step<D, SRC, true>(st, tX, tO, i == 0, max(f.n, 0), sk, f.sv, product_done, turns);
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -1166,6 +1198,9 @@ static int launch_pairs(Args a, const uint16_t* const (&kv)[2], const int64_t (&
     if (int rc = make_map(&v, kv[1], a.keys, n, D, ld[1], hs[1], kSeg)) return rc;
     const int64_t items = (SRC == kWide ? cdiv(a.nq, 2) * a.heads : cdiv(a.nq * a.heads, 2)) * a.parts;
     a.items = (uint32_t)items;
+    // Turns pay where items are long (64 steps: 1.02 ms instead of 1.11) and cost where a tile's output keeps the
+    // other waiting every few steps (8 steps: 1.68 ms instead of 1.59).
+    a.turns = a.segs / a.parts >= 24;
     H3B_CUDA_TRY(cudaFuncSetAttribute(pair_kernel<D, SRC>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::kBytes));
     const int64_t grid = items < sm_count() ? items : sm_count();
     pair_kernel<D, SRC><<<(unsigned)grid, kPairThreads, Smem<D>::kBytes, s>>>(q, k, v, o, a);
