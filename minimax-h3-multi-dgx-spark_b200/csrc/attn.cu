@@ -56,7 +56,6 @@ struct Args {
 
 constexpr int kTmemCols = 512;     // S of tile t at 128 t (+ 64 for odd steps), O at 256 + 128 t
 constexpr int kPairThreads = 384;  // 2 x 4 softmax warps, an MMA warp and a TMA warp for each tile
-constexpr uint64_t kWaitNs = 1000ull * 1000 * 1000;
 constexpr float kLog2e = 1.4426950408889634f;
 // A row's reference maximum moves when a score exceeds it by 2^8: until then p
 // stays below 2^8, far from any limit of fp32 or bf16 (whose relative
@@ -251,7 +250,7 @@ __device__ __forceinline__ bool await(uint64_t* bar, uint32_t phase, volatile in
         if (*abort_flag) return false;
         const uint64_t now = globaltimer_ns();
         if (!t0) t0 = now;
-        if (now - t0 > kWaitNs) {
+        if (now - t0 > kTimeoutNs) {
             *abort_flag = 1;
             report(status, H3B_STATUS_MBAR_TIMEOUT);
             return false;
@@ -1308,7 +1307,7 @@ extern "C" int h3b_block_sparse_attn(const void* q, int64_t q_ld, int64_t q_hs, 
                                      int64_t v_hs, int64_t Sk, const int32_t* blocks, int64_t topk, float scale,
                                      void* o, int64_t o_ld, int64_t o_hs, void* workspace, int64_t workspace_bytes,
                                      void* stream) {
-    H3B_REQUIRE(topk >= 0 && topk < (1ll << 31) && H > 0 && H <= 65535, "h3b_block_sparse_attn: topk=%lld heads=%lld out of range",
+    H3B_REQUIRE(topk >= 0 && topk <= (1ll << 25) && H > 0 && H <= 65535, "h3b_block_sparse_attn: topk=%lld heads=%lld out of range",
                 (long long)topk, (long long)H);
     H3B_REQUIRE(topk == 0 || (blocks && aligned(blocks, 4)), "h3b_block_sparse_attn: blocks NULL");
     H3B_REQUIRE(Sk == 0 || (k && v && aligned(k, 16) && aligned(v, 16)),

@@ -72,6 +72,7 @@ def test_attention_refusals():
         return lib.h3b_block_sparse_attn(P16, 128, 128, 1, 1, D, k, kld, 128, P16, 128, 128, Sk, blocks, topk, 1.0, P16,
                                          128, 128, P0, 0, P0)
     refused("h3b_block_sparse_attn", sparse(topk=-1), "topk")
+    refused("h3b_block_sparse_attn", sparse(topk=2 ** 26), "topk")
     refused("h3b_block_sparse_attn", sparse(blocks=P0), "blocks")
     refused("h3b_block_sparse_attn", sparse(k=P2), "aligned")
     refused("h3b_block_sparse_attn", sparse(kld=4), "strides")

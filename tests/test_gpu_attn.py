@@ -533,3 +533,46 @@ def test_sparse_attention_over_many_items(rows, H):
     ref, a, m = sparse(q[:, heads], k[:, heads], v[:, heads], blocks[heads], 64 ** -0.5)
     near(o[:, heads], ref, a, m, 192, 64)
     assert h3b.status() == 0
+
+
+def test_cached_attention_widens_its_heads_in_groups():
+    """Codes of 5 heads that widen to 360 MB: more than the workspace takes at a time."""
+    H, n, D, rows = 5, 140000, 128, 70
+    c = filled(H, -(-n // 64) * 64, D, n, seed=31)
+    assert 2 * n * D * 2 * H > 256 << 20
+    q = randn(rows, H, D, seed=32)
+    got = h3b.kv8_attention(q, c)
+    k, v = values(c)
+    for h in range(H):
+        o, a, m = softmax_rows(q[:, h], k[:, h], v[:, h], D ** -0.5)
+        near(got[:, h], o, a, m, n, D)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows,H,topk", [(300, 3, 40), (128, 1, 70), (513, 60, 30)])
+def test_sparse_attention_over_long_lists(D, rows, H, topk):
+    """Items of 24 steps or more, whose tiles' exponentials take turns, with and without a tile at the end that has no
+    partner."""
+    q, k, v = randn(rows, H, D, seed=1), randn(5000, H, D, seed=2), randn(5000, H, D, seed=3)
+    o, blocks = h3b.sparse_attention(q, k, v, topk, return_blocks=True)
+    heads = sorted({0, H // 2, H - 1})
+    ref, a, m = sparse(q[:, heads], k[:, heads], v[:, heads], blocks[heads], D ** -0.5)
+    near(o[:, heads], ref, a, m, topk * 64, D)
+    assert h3b.status() == 0
+
+
+@pytest.mark.parametrize("rows,tokens,H", [(16000, 512, 4), (1000, 64, 40), (700, 4000, 7), (200, 129, 3)])
+def test_repeated_calls_are_bitwise_equal(rows, tokens, H):
+    """Nothing depends on which of the kernel's warps comes first: fifty runs, other work on another stream meanwhile."""
+    c = filled(H, -(-tokens // 64) * 64, 128, tokens, seed=41)
+    q = randn(rows, H, 128, seed=42)
+    want = h3b.kv8_attention(q, c)
+    sq = h3b.sparse_attention(q, q, q, 5)
+    side = torch.cuda.Stream()
+    a = randn(2048, 2048, seed=43)
+    torch.cuda.synchronize()
+    for _ in range(50):
+        with torch.cuda.stream(side):
+            a @ a
+        assert torch.equal(h3b.kv8_attention(q, c), want) and torch.equal(h3b.sparse_attention(q, q, q, 5), sq)
+    assert h3b.status() == 0
