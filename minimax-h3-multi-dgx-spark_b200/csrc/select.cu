@@ -6,43 +6,76 @@
 // add up exactly there) and rounded once to 32 bits; scores are sums of exact
 // products in 64 bits; equal scores go to the lowest index.  A NaN score ranks
 // below every number, -0 equals +0.
-#include "common.cuh"
+#include "quant_common.cuh"
 
 namespace h3b {
 namespace sel {
 
 constexpr int kThreads = 256;
 
-// mean over the rows of a block of x [S, H, D] -> out [nb, H, D] fp32.
-// One CTA per (block, head); 8 channels a thread, kThreads / (D / 8) row lanes.
-// Bound by its reads; a whole block's loads are all in flight before the first
-// conversion to 64 bits.
+// bf16 -> fp64 times 2^-896 without a conversion instruction (of which an SM does
+// too few to keep up with its reads): the exponent and mantissa moved into place,
+// which holds for subnormal values as well; infinities and NaNs need the exact
+// conversion.  Sums of such values are the exact conversions' sums scaled.
+__device__ __forceinline__ double scaled_lo(uint32_t w) {
+    return __hiloint2double(((int)(w << 16) >> 3) & 0x8FFFFFFF, 0);
+}
+__device__ __forceinline__ double scaled_hi(uint32_t w) { return __hiloint2double(((int)w >> 3) & 0x8FFFE000, 0); }
+constexpr double kDown = 0x1p-896, kUp = 0x1p896;
+
+struct Means {
+    const uint16_t* x;  // [S, H, D]
+    int64_t ld, hs, S;
+    float* out;  // [nb, H, D]
+    int64_t ctas;  // blocks x heads
+};
+
+// More bytes in flight for its registers than 256 threads with half the rows each.
+constexpr int kMeanThreads = 128;
+
+// mean over the rows of a block of x -> fp32, one CTA per (block, head); 8
+// channels a thread, kMeanThreads / (D / 8) row lanes.  Bound by its reads; a whole
+// block's loads are in flight before the first is used.
 template <int D, int ROWS>
-__global__ void __launch_bounds__(kThreads) means_kernel(const uint16_t* __restrict__ x, int64_t ld, int64_t hs,
-                                                         int64_t S, int H, float* __restrict__ out) {
+__device__ __forceinline__ void block_mean(const Means& a, int H, int64_t cta) {
     constexpr int kCols = D / 8;
-    constexpr int kRows = kThreads / kCols;
+    constexpr int kRows = kMeanThreads / kCols;
     constexpr int kLoads = ROWS / kRows;
-    constexpr int kWarps = kThreads / 32;
-    const int h = (int)(blockIdx.x % (unsigned)H);
-    const int64_t b = blockIdx.x / (unsigned)H;
+    constexpr int kWarps = kMeanThreads / 32;
+    const int64_t b = (int64_t)((uint32_t)cta / (uint32_t)H);
+    const int h = (int)((uint32_t)cta - (uint32_t)b * (uint32_t)H);
     const int col = threadIdx.x % kCols, row = threadIdx.x / kCols;
-    const int count = (int)min((int64_t)ROWS, S - b * ROWS);
-    const uint16_t* src = x + (b * ROWS + row) * ld + h * hs + col * 8;
+    const int count = (int)min((int64_t)ROWS, a.S - b * ROWS);
+    const uint16_t* src = a.x + (b * ROWS + row) * a.ld + h * a.hs + col * 8;
     uint4 v[kLoads];
 #pragma unroll
     for (int p = 0; p < kLoads; ++p) {
         v[p] = make_uint4(0, 0, 0, 0);
-        if (row + p * kRows < count) v[p] = __ldcs(reinterpret_cast<const uint4*>(src + (int64_t)p * kRows * ld));
+        if (row + p * kRows < count) v[p] = __ldcs(reinterpret_cast<const uint4*>(src + (int64_t)p * kRows * a.ld));
     }
     double acc[8] = {};
+    uint32_t top = 0;  // largest |x| of the low and of the high halves
 #pragma unroll
-    for (int p = 0; p < kLoads; ++p) {
-        const uint32_t w[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
+    for (int p = 0; p < kLoads; ++p) top = absmax_bits8(v[p], top);
+    if (max(top & 0xFFFFu, top >> 16) < 0x7F80u) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            acc[2 * e] += (double)bf16_lo(w[e]);
-            acc[2 * e + 1] += (double)bf16_hi(w[e]);
+        for (int p = 0; p < kLoads; ++p) {
+            const uint32_t w[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                acc[2 * e] += scaled_lo(w[e]);
+                acc[2 * e + 1] += scaled_hi(w[e]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int p = 0; p < kLoads; ++p) {
+            const uint32_t w[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                acc[2 * e] += (double)bf16_lo(w[e]) * kDown;
+                acc[2 * e + 1] += (double)bf16_hi(w[e]) * kDown;
+            }
         }
     }
     // the row lanes of a warp, then the warps
@@ -54,32 +87,63 @@ __global__ void __launch_bounds__(kThreads) means_kernel(const uint16_t* __restr
         if (threadIdx.x % 32 < kCols) part[threadIdx.x / 32][col * 8 + e] = acc[e];
     }
     __syncthreads();
-    if (threadIdx.x < D) {
+    for (int ch = threadIdx.x; ch < D; ch += kMeanThreads) {
         double t = 0.0;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) t += part[w][threadIdx.x];
-        out[(b * H + h) * D + threadIdx.x] = (float)(t / (double)count);
+        for (int w = 0; w < kWarps; ++w) t += part[w][ch];
+        a.out[(b * H + h) * D + ch] = (float)(t * kUp / (double)count);
     }
+}
+
+// Blocks of 64 rows of one tensor and of 128 rows of another (either may have none).
+template <int D>
+__global__ void __launch_bounds__(kMeanThreads) means_kernel(const __grid_constant__ Means by64,
+                                                         const __grid_constant__ Means by128, int H) {
+    if (blockIdx.x < by64.ctas) block_mean<D, 64>(by64, H, blockIdx.x);
+    else block_mean<D, 128>(by128, H, blockIdx.x - by64.ctas);
+}
+
+static int launch_means(const Means& by64, const Means& by128, int64_t H, int64_t D, cudaStream_t s) {
+    const unsigned grid = (unsigned)(by64.ctas + by128.ctas);
+    if (grid == 0) return H3B_OK;
+    if (D == 128) means_kernel<128><<<grid, kMeanThreads, 0, s>>>(by64, by128, (int)H);
+    else means_kernel<64><<<grid, kMeanThreads, 0, s>>>(by64, by128, (int)H);
+    H3B_CUDA_TRY(cudaGetLastError());
+    return H3B_OK;
+}
+
+static int check_means(const char* who, const void* x, int64_t ld, int64_t hs, int64_t S, int64_t H, int64_t rows,
+                       float* out, Means* m) {
+    *m = Means{static_cast<const uint16_t*>(x), ld, hs, S, out, cdiv(S, rows) * H};
+    if (S == 0) return H3B_OK;
+    H3B_REQUIRE(x && out && aligned(x, 16) && ld % 8 == 0 && hs % 8 == 0,
+                "%s: x / out NULL, x not 16-byte aligned or strides not multiples of 8 elements", who);
+    H3B_REQUIRE(m->ctas < (1ll << 30), "%s: too many blocks", who);
+    return H3B_OK;
 }
 
 constexpr int kTile = 64;  // query rows (and key blocks) per score tile
 constexpr int kFew = 4;    // query blocks up to which the scores are plain products
 
 // score[unit][i][j] = sum_d qm[i, h, d] * km[j, h, d] in 64 bits, one unit
-// being 64 query blocks of a head.  Four warps a tile of 64 x 64, each 32 x 32 by
-// mma.sync m8n8k4 in fp64; both operands lie in shared memory as fp32, their
-// whole depth at once.  Bound by the fp64 products.
-template <int D>
+// being 64 query blocks of a head.  Four warps a tile of T x T by mma.sync m8n8k4
+// in fp64; both operands lie in shared memory as fp32, their whole depth at once.
+// Bound by the fp64 products with T = 64; T = 32 where there are too few such
+// tiles for the SMs (33 x 65 blocks of 40 heads).
+template <int D, int T>
 __global__ void __launch_bounds__(128) score_kernel(const float* __restrict__ qm, const float* __restrict__ km, int nq,
                                                     int64_t nk, int H, int tiles, int64_t unit0,
                                                     double* __restrict__ score) {
     constexpr int kLd = D + 4;  // 8 rows x 4 channels of an operand meet 32 banks
     extern __shared__ __align__(16) float tile[];
-    float *qs = tile, *ks = tile + kTile * kLd;
-    const int64_t unit = unit0 + blockIdx.y;
+    float *qs = tile, *ks = tile + T * kLd;
+    constexpr int kSub = kTile / T;  // tiles down a unit
+    const int64_t unit = unit0 + blockIdx.y / kSub;
+    const int sub = blockIdx.y % kSub * T;
     const int h = (int)(unit / tiles);
-    const int64_t i0 = (unit % tiles) * kTile, j0 = (int64_t)blockIdx.x * kTile;
-    for (int e = threadIdx.x; e < kTile * (D / 4); e += 128) {
+    const int64_t i0 = (unit % tiles) * kTile + sub, j0 = (int64_t)blockIdx.x * T;
+    if (i0 >= nq) return;
+    for (int e = threadIdx.x; e < T * (D / 4); e += 128) {
         const int r = e / (D / 4), d = e % (D / 4) * 4;
         float4 x = make_float4(0, 0, 0, 0), y = x;
         if (i0 + r < nq) x = *reinterpret_cast<const float4*>(qm + ((i0 + r) * H + h) * D + d);
@@ -89,34 +153,35 @@ __global__ void __launch_bounds__(128) score_kernel(const float* __restrict__ qm
     }
     __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int wi = (warp >> 1) * 32, wj = (warp & 1) * 32;
+    constexpr int E = T / 16;  // products of 8 x 8 along a warp's side
+    const int wi = (warp >> 1) * (T / 2), wj = (warp & 1) * (T / 2);
     const float* qa = qs + (wi + (lane >> 2)) * kLd + (lane & 3);
     const float* ka = ks + (wj + (lane >> 2)) * kLd + (lane & 3);
-    double acc[4][4][2] = {};
+    double acc[E][E][2] = {};
 #pragma unroll 4
     for (int d = 0; d < D; d += 4) {
-        double x[4], y[4];
+        double x[E], y[E];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < E; ++e) {
             x[e] = (double)qa[e * 8 * kLd + d];
             y[e] = (double)ka[e * 8 * kLd + d];
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < E; ++e)
 #pragma unroll
-            for (int f = 0; f < 4; ++f)
+            for (int f = 0; f < E; ++f)
                 asm("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0, %1}, {%2}, {%3}, {%0, %1};"
                     : "+d"(acc[e][f][0]), "+d"(acc[e][f][1])
                     : "d"(x[e]), "d"(y[f]));
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < E; ++e)
 #pragma unroll
-        for (int f = 0; f < 4; ++f)
+        for (int f = 0; f < E; ++f)
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int64_t j = j0 + wj + 8 * f + 2 * (lane & 3) + k;
-                if (j < nk) score[((int64_t)blockIdx.y * kTile + wi + 8 * e + (lane >> 2)) * nk + j] = acc[e][f][k];
+                if (j < nk) score[((int64_t)(blockIdx.y / kSub) * kTile + sub + wi + 8 * e + (lane >> 2)) * nk + j] = acc[e][f][k];
             }
 }
 
@@ -326,10 +391,16 @@ static int scores(const float* qm, const float* km, int nq, int64_t nk, int H, i
         const dim3 grid((unsigned)cdiv(nk, kThreads / 32), (unsigned)units);
         score_few_kernel<D><<<grid, kThreads, 0, s>>>(qm, km, nq, nk, H, unit, score);
     } else {
-        constexpr int smem = 2 * kTile * (D + 4) * 4;
-        H3B_CUDA_TRY(cudaFuncSetAttribute(score_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        const dim3 grid((unsigned)cdiv(nk, kTile), (unsigned)units);
-        score_kernel<D><<<grid, 128, smem, s>>>(qm, km, nq, nk, H, tiles, unit, score);
+        const int64_t big = cdiv(nk, kTile) * units;
+        constexpr int smem64 = 2 * 64 * (D + 4) * 4, smem32 = 2 * 32 * (D + 4) * 4;
+        if (big >= 2 * 148) {  // two a SM
+            H3B_CUDA_TRY(cudaFuncSetAttribute(score_kernel<D, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem64));
+            score_kernel<D, 64><<<dim3((unsigned)cdiv(nk, 64), (unsigned)units), 128, smem64, s>>>(qm, km, nq, nk, H, tiles,
+                                                                                                unit, score);
+        } else {
+            score_kernel<D, 32><<<dim3((unsigned)cdiv(nk, 32), (unsigned)(2 * units)), 128, smem32, s>>>(
+                qm, km, nq, nk, H, tiles, unit, score);
+        }
     }
     H3B_CUDA_TRY(cudaGetLastError());
     return H3B_OK;
@@ -346,20 +417,24 @@ extern "C" int h3b_block_means(const void* x, int64_t ld, int64_t hs, int64_t S,
     H3B_REQUIRE(S >= 0 && H > 0 && H <= 65535 && (rows == 64 || rows == 128),
                 "h3b_block_means: S=%lld heads=%lld rows=%lld (64 or 128) out of range", (long long)S, (long long)H,
                 (long long)rows);
-    if (S == 0) return H3B_OK;
-    H3B_REQUIRE(x && out && aligned(x, 16) && ld % 8 == 0 && hs % 8 == 0,
-                "h3b_block_means: x / out NULL, x not 16-byte aligned or strides not multiples of 8 elements");
-    H3B_REQUIRE(cdiv(S, rows) * H < (1ll << 31), "h3b_block_means: too many blocks");
-    const unsigned grid = (unsigned)(cdiv(S, rows) * H);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const uint16_t* p = static_cast<const uint16_t*>(x);
-    if (D == 128 && rows == 128) sel::means_kernel<128, 128><<<grid, sel::kThreads, 0, s>>>(p, ld, hs, S, (int)H, out);
-    else if (D == 128) sel::means_kernel<128, 64><<<grid, sel::kThreads, 0, s>>>(p, ld, hs, S, (int)H, out);
-    else if (rows == 128) sel::means_kernel<64, 128><<<grid, sel::kThreads, 0, s>>>(p, ld, hs, S, (int)H, out);
-    else sel::means_kernel<64, 64><<<grid, sel::kThreads, 0, s>>>(p, ld, hs, S, (int)H, out);
-    H3B_CUDA_TRY(cudaGetLastError());
-    return H3B_OK;
+    sel::Means m, none{};
+    if (int rc = sel::check_means("h3b_block_means", x, ld, hs, S, H, rows, out, &m)) return rc;
+    return rows == 64 ? sel::launch_means(m, none, H, D, static_cast<cudaStream_t>(stream))
+                      : sel::launch_means(none, m, H, D, static_cast<cudaStream_t>(stream));
 }
+
+// Means of 64 keys and of 128 query rows in one launch (sparse.cu).
+namespace h3b {
+int sparse_means(const void* k, int64_t k_ld, int64_t k_hs, int64_t Sk, float* km, const void* q, int64_t q_ld,
+                 int64_t q_hs, int64_t Sq, float* qm, int64_t H, int64_t D, cudaStream_t s) {
+    sel::Means a{}, b;
+    if (km) {
+        if (int rc = sel::check_means("h3b_sparse_attn", k, k_ld, k_hs, Sk, H, 64, km, &a)) return rc;
+    }
+    if (int rc = sel::check_means("h3b_sparse_attn", q, q_ld, q_hs, Sq, H, 128, qm, &b)) return rc;
+    return sel::launch_means(a, b, H, D, s);
+}
+}  // namespace h3b
 
 extern "C" int64_t h3b_select_blocks_workspace(int64_t nq, int64_t nk, int64_t H) {
     if (nq <= 0 || nk <= 0 || H <= 0) return 0;

@@ -2,6 +2,11 @@
 // selection and the attention over it, enqueued one behind the other.
 #include "common.cuh"
 
+namespace h3b {
+int sparse_means(const void* k, int64_t k_ld, int64_t k_hs, int64_t Sk, float* km, const void* q, int64_t q_ld,
+                 int64_t q_hs, int64_t Sq, float* qm, int64_t H, int64_t D, cudaStream_t s);
+}  // namespace h3b
+
 using namespace h3b;
 
 namespace {
@@ -54,10 +59,9 @@ extern "C" int h3b_sparse_attn(const void* q, int64_t q_ld, int64_t q_hs, int64_
     char* ws = static_cast<char*>(workspace);
     float *qm = reinterpret_cast<float*>(ws + l.qm), *km = reinterpret_cast<float*>(ws + l.km);
     if (l.topk > 0 && Sq > 0) {
-        if (!k_means) {
-            if (int rc = h3b_block_means(k, k_ld, k_hs, Sk, H, D, kKeys, km, stream)) return rc;
-        }
-        if (int rc = h3b_block_means(q, q_ld, q_hs, Sq, H, D, kQRows, qm, stream)) return rc;
+        if (int rc = sparse_means(k, k_ld, k_hs, Sk, k_means ? nullptr : km, q, q_ld, q_hs, Sq, qm, H, D,
+                                  static_cast<cudaStream_t>(stream)))
+            return rc;
         if (int rc = h3b_select_blocks(qm, k_means ? k_means : km, l.nq, l.nk, H, D, l.topk, blocks, ws + l.select,
                                        workspace_bytes - l.select, stream))
             return rc;

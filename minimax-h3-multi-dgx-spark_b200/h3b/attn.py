@@ -287,7 +287,7 @@ def sparse_attention(q, k, v, topk, scale=None, k_means=None, return_blocks=Fals
         has = int(k_means is not None)
         nbytes = lib.h3b_sparse_attn_workspace(sq, sk, H, D, topk, has)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        with _on(q.device), span("sparse_attn", 4.0 * sq * topk * KEYS * H * D, launches=5 - has):
+        with _on(q.device), span("sparse_attn", 4.0 * sq * topk * KEYS * H * D, launches=4):
             check(lib.h3b_sparse_attn(_ptr(q), qld, qhs, sq, H, D, _ptr(k), kld, khs, _ptr(v), vld, vhs, sk, _ptr(k_means),
                                       topk, _scale(scale, D), _ptr(blocks), _ptr(o), H * D, D, _ptr(ws), nbytes,
                                       _stream(q.device)), "h3b_sparse_attn")

@@ -90,7 +90,7 @@ def test_sparse_attention_refusals():
     refused("h3b_sparse_attn", sparse(topk=-1), "topk")
     refused("h3b_sparse_attn", sparse(ws=P0), "workspace")
     refused("h3b_sparse_attn", sparse(size=100), "workspace")
-    refused("h3b_block_means", sparse(k=P2), "aligned")
+    refused("h3b_sparse_attn", sparse(k=P2), "aligned")
     # query means, key means (unless kept) and the scores
     assert lib.h3b_sparse_attn_workspace(200, 100, 2, 128, 2, 0) == 2048 + 2048 + 2 * 64 * 2 * 8
     assert lib.h3b_sparse_attn_workspace(200, 100, 2, 128, 2, 1) == 2048 + 2 * 64 * 2 * 8
