@@ -770,7 +770,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 constexpr int kRowWarps = 4, kRowWarpsMost = 8;
 constexpr float kRowSlack = 4.0f, kRowBias = 11.0f;
 // Up to this many rows the rows kernel reads the codes once per 16 rows (from L2
-// after the first); beyond, they are widened once for the pair kernel.
+// after the first); beyond, they are widened once for the pair kernel (64 rows
+// over 16384 tokens of 40 heads: 195 us and 211).
 constexpr int64_t kRowsMost = 64;
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -797,7 +798,7 @@ __device__ __forceinline__ uint32_t half_codes(uint32_t x) {
     return *reinterpret_cast<const uint32_t*>(&d);
 }
 
-// CTAs an SM: as many as the registers allow without spilling (three instead of
+// CTAs an SM: as many as the registers allow almost without spilling (three instead of
 // two: 0.248 ms instead of 0.302 for a row over 131071 tokens of 40 heads).
 constexpr int row_ctas(int64_t D, int groups) { return groups == 2 ? 2 : D == 128 ? 3 : 4; }
 
@@ -1182,7 +1183,11 @@ static Plan plan(bool cache, int64_t Sq, int64_t H, int64_t D, int64_t segs) {
     }
     const int64_t nq = cdiv(Sq, kQRows);
     const int64_t head = cache ? 2 * segs * kSeg * D * 2 : 0;
-    if (H * head > kWideBytes) p.heads = kWideBytes / head > 0 ? kWideBytes / head : 1;
+    if (H * head > kWideBytes) {
+        // as few launches as that allows, of about as many heads each (16 and 4 heads: 1.05 ms, 10 and 10: 0.85)
+        const int64_t most = kWideBytes / head > 0 ? kWideBytes / head : 1;
+        p.heads = cdiv(H, cdiv(H, most));
+    }
     p.parts = parts_of(cache, nq, p.heads, segs);
     p.join_at = p.heads * head;
     p.bytes = p.join_at + (p.parts > 1 ? p.parts * p.heads * Sq * (D + 2) * 4 : 0);

@@ -576,3 +576,11 @@ def test_repeated_calls_are_bitwise_equal(rows, tokens, H):
             a @ a
         assert torch.equal(h3b.kv8_attention(q, c), want) and torch.equal(h3b.sparse_attention(q, q, q, 5), sq)
     assert h3b.status() == 0
+
+
+@pytest.mark.parametrize("rows", [8, 9, 64, 65])
+@pytest.mark.parametrize("tokens", [200, 3000])
+def test_cached_attention_where_the_kernels_change(rows, tokens):
+    """Row counts on both sides of each choice of kernel: a row's output does not depend on it beyond its rounding."""
+    c = filled(3, -(-tokens // 64) * 64, 128, tokens, seed=rows)
+    check_cached(randn(rows, 3, 128, seed=tokens), c)
