@@ -276,7 +276,7 @@ H3B_API int h3b_kv8_read(const int8_t *kq, const int8_t *vq, const float *ks, co
  * needed, NULL will do): h3b_kv8_attn with `cache` set and segments =
  * ceil(length / 64), h3b_block_sparse_attn with cache 0 and segments = topk.
  * With few row tiles the keys are split over CTAs, whose parts meet there; with
- * many, a cache's codes are widened to bf16 there once (at most 256 MiB of
+ * many, a cache's codes are widened to bf16 there once (at most 512 MiB of
  * heads, or one head, at a time).  Calls that may overlap need workspaces of
  * their own.  The reference's attention call is at sp_forward.py:276-318. */
 H3B_API int64_t h3b_attn_workspace(int cache, int64_t Sq, int64_t H, int64_t D, int64_t segments);

@@ -771,7 +771,8 @@ constexpr int kRowWarps = 4, kRowWarpsMost = 8;
 constexpr float kRowSlack = 4.0f, kRowBias = 11.0f;
 // Up to this many rows the rows kernel reads the codes once per 16 rows (from L2
 // after the first); beyond, they are widened once for the pair kernel (64 rows
-// over 16384 tokens of 40 heads: 195 us and 211).
+// over 16384 tokens of 40 heads: 190 us and 180; over 60000 of 10: 160 and 162;
+// over 512 of 40: 25 and 35; 48 rows over 16384 of 40: 153 and 180).
 constexpr int64_t kRowsMost = 64;
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -1167,7 +1168,8 @@ struct Plan {
     int64_t join_at, bytes;  // in the workspace
 };
 
-constexpr int64_t kWideBytes = 256ll << 20;  // of widened heads at a time (one head at least)
+// of widened heads at a time (one head at least): 256 rows over 16384 tokens of 40 heads 211 us, with 256 MiB 227
+constexpr int64_t kWideBytes = 512ll << 20;
 
 static Plan plan(bool cache, int64_t Sq, int64_t H, int64_t D, int64_t segs) {
     Plan p{false, 0, H, 1, 0, 0};

@@ -64,7 +64,7 @@ def test_attention_refusals():
     refused("h3b_kv8_attn", cached(cap=4096, length=4096), "workspace")
     assert lib.h3b_attn_workspace(1, 1, 1, 128, 64) > 0 and lib.h3b_attn_workspace(1, 0, 1, 128, 64) == 0
     assert lib.h3b_attn_workspace(0, 100000, 40, 128, 64) == 0 and lib.h3b_attn_workspace(1, 5, 1, 128, 0) == 0
-    # a cache's widened heads: 256 MiB at most, or one head
+    # a cache's widened heads: 512 MiB at most, or one head
     assert lib.h3b_attn_workspace(1, 100000, 40, 128, 1 << 14) >= 2 ** 20 * 512
     assert cached(Sq=0) == 0
 
