@@ -650,7 +650,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 const Seg g = segment<SRC>(a, list, it.step0 + i);
                 if (SRC == kBlocks) return Factors{g.n, scale2, 1.0f};
                 const int64_t b = (int64_t)(a.h0 + u.h) * (a.cap / kSeg) + it.step0 + i;
-                return Factors{g.n, __ldg(a.scales[0] + b), __ldg(a.scales[1] + b)};
+                return Factors{g.n, fabsf(__ldg(a.scales[0] + b)), __ldg(a.scales[1] + b)};  // (signs: widen_kernel)
             };
             Factors ahead = factors(0);
             const bool paired = it.both && a.turns;
@@ -1085,27 +1085,36 @@ __global__ void __launch_bounds__(256) zero_kernel(Args a, int per_head, int64_t
     *reinterpret_cast<uint4*>(a.o + row / a.H * a.o_ld + row % a.H * a.o_hs + i % per_head * 8) = make_uint4(0, 0, 0, 0);
 }
 
-// Codes of some heads (each `per` pieces of 16 from `stride` pieces apart) -> bf16, K or V by blockIdx.y.
+// Codes of some heads (each `per` pieces of 16 from `stride` pieces apart) -> bf16, K or V by blockIdx.y.  A key
+// scale's sign goes into the codes (2^block_log2 pieces share a scale): the maximum of a block's scores is taken
+// before its scale, which must not turn their order.  (Turning the scores there costs the long kernel 2%.)
 __global__ void __launch_bounds__(256) widen_kernel(const int8_t* __restrict__ kq, const int8_t* __restrict__ vq,
-                                                    int64_t stride, int64_t per, int64_t pieces,
+                                                    const float* __restrict__ ks, int64_t stride, int64_t per,
+                                                    int64_t pieces, int block_log2,
                                                     uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
     const uint4* src = reinterpret_cast<const uint4*>(blockIdx.y ? vq : kq);
     uint4* dst = reinterpret_cast<uint4*>(blockIdx.y ? v : k);
     uint4 x[4];
+    uint32_t sign[4];
     const int64_t first = (int64_t)blockIdx.x * 1024 + threadIdx.x;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         const int64_t i = first + p * 256;
-        if (i < pieces) x[p] = __ldg(src + i / per * stride + i % per);
+        if (i >= pieces) break;
+        const int64_t at = i / per * stride + i % per;
+        x[p] = __ldg(src + at);
+        sign[p] = blockIdx.y == 0 && __ldg(ks + (at >> block_log2)) < 0.0f ? 0x80008000u : 0u;
     }
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         const int64_t i = first + p * 256;
         if (i >= pieces) break;
-        dst[2 * i] = make_uint4(codes_to_bf16x2(x[p].x, 0x4140), codes_to_bf16x2(x[p].x, 0x4342),
-                                codes_to_bf16x2(x[p].y, 0x4140), codes_to_bf16x2(x[p].y, 0x4342));
-        dst[2 * i + 1] = make_uint4(codes_to_bf16x2(x[p].z, 0x4140), codes_to_bf16x2(x[p].z, 0x4342),
-                                    codes_to_bf16x2(x[p].w, 0x4140), codes_to_bf16x2(x[p].w, 0x4342));
+        const uint32_t w[4] = {x[p].x, x[p].y, x[p].z, x[p].w};
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            dst[2 * i + e] = make_uint4(
+                codes_to_bf16x2(w[2 * e], 0x4140) ^ sign[p], codes_to_bf16x2(w[2 * e], 0x4342) ^ sign[p],
+                codes_to_bf16x2(w[2 * e + 1], 0x4140) ^ sign[p], codes_to_bf16x2(w[2 * e + 1], 0x4342) ^ sign[p]);
     }
 }
 
@@ -1240,7 +1249,8 @@ static int launch_all(Args& a, bool cache, const Plan& p, char* ws, cudaStream_t
         uint16_t* const v = k + n * rows * D;
         const int64_t pieces = n * rows * D / 16;
         widen_kernel<<<dim3((unsigned)cdiv(pieces, 4 * 256), 2), 256, 0, s>>>(
-            a.codes[0] + h * a.cap * D, a.codes[1] + h * a.cap * D, a.cap * D / 16, rows * D / 16, pieces, k, v);
+            a.codes[0] + h * a.cap * D, a.codes[1] + h * a.cap * D, a.scales[0] + h * (a.cap / kSeg), a.cap * D / 16,
+            rows * D / 16, pieces, D == 128 ? 9 : 8, k, v);
         a.h0 = (int)h;
         a.heads = (int)n;
         const int64_t ld[2] = {D, D}, hs[2] = {rows * D, rows * D};

@@ -584,3 +584,23 @@ def test_cached_attention_where_the_kernels_change(rows, tokens):
     """Row counts on both sides of each choice of kernel: a row's output does not depend on it beyond its rounding."""
     c = filled(3, -(-tokens // 64) * 64, 128, tokens, seed=rows)
     check_cached(randn(rows, 3, 128, seed=tokens), c)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows", [1, 20, 300])
+def test_cached_attention_over_negative_scales(D, rows):
+    """Scales of a wrapped cache may be of either sign, and zero."""
+    c = filled(3, 704, D, 650, seed=51)
+    sign = torch.tensor([1.0, -1.0, -1.0, 0.0, 1.0, -1.0, 1.0, 1.0, -1.0, 0.0, -1.0], device=DEV)
+    c.ks.mul_(sign)
+    c.vs.mul_(sign.flip(0))
+    check_cached(randn(rows, 3, D, seed=52, scale=4.0), c)
+    check_cached(randn(rows, 3, D, seed=53, scale=4.0), c, scale=-0.2)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
+@pytest.mark.parametrize("rows,topk", [(1, 3), (300, 3), (300, 40)])
+def test_sparse_attention_of_other_scales(rows, topk, scale):
+    q, k, v = randn(rows, 3, 128, seed=54), randn(2700, 3, 128, seed=55), randn(2700, 3, 128, seed=56)
+    blocks = h3b.select_blocks(h3b.block_means(q, 128), h3b.block_means(k), topk)
+    check_sparse(q, k, v, blocks, scale)
