@@ -650,7 +650,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 const Seg g = segment<SRC>(a, list, it.step0 + i);
                 if (SRC == kBlocks) return Factors{g.n, scale2, 1.0f};
                 const int64_t b = (int64_t)(a.h0 + u.h) * (a.cap / kSeg) + it.step0 + i;
-                return Factors{g.n, fabsf(__ldg(a.scales[0] + b)), __ldg(a.scales[1] + b)};  // (signs: widen_kernel)
+                // (the scores' signs: widen_kernel; a cache of one block has its values' scale in the output)
+                return Factors{g.n, fabsf(__ldg(a.scales[0] + b)), a.segs == 1 ? 1.0f : __ldg(a.scales[1] + b)};
             };
             Factors ahead = factors(0);
             const bool paired = it.both && a.turns;
@@ -682,7 +683,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             tc_fence_after();
             const int64_t row = (int64_t)u.qt * kQRows + trow;
             const bool split = a.parts > 1;
-            const float inv = st.l == 0.0f ? 0.0f : 1.0f / st.l;
+            float inv = st.l == 0.0f ? 0.0f : 1.0f / st.l;
+            // (one block: its scale is not rounded with p, whose rounding would be that of every output of a head where
+            // there is one token)
+            if (SRC == kWide && a.segs == 1) inv *= __ldg(a.scales[1] + (int64_t)(a.h0 + u.h) * (a.cap / kSeg));
             const int64_t slot = ((int64_t)it.part * a.heads + u.h) * a.Sq + row;
             if (split && row < a.Sq) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(st.m, st.l);
             // the output's place is free when the store before has read it

@@ -604,3 +604,14 @@ def test_sparse_attention_of_other_scales(rows, topk, scale):
     q, k, v = randn(rows, 3, 128, seed=54), randn(2700, 3, 128, seed=55), randn(2700, 3, 128, seed=56)
     blocks = h3b.select_blocks(h3b.block_means(q, 128), h3b.block_means(k), topk)
     check_sparse(q, k, v, blocks, scale)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows", [65, 300])
+def test_cached_attention_to_a_single_token_rounds_once(D, rows):
+    """p and its sum are 1 up to 2^-24 of a score's reference (below 2^6 here), so the output is the token's value
+    rounded to bf16: half a step and less than 2^-16 beside it."""
+    c = filled(5, 64, D, 1, seed=61)
+    got = h3b.kv8_attention(randn(rows, 5, D, seed=62), c).double()
+    want = values(c)[1].expand(rows, -1, -1)
+    assert ((got - want).abs() <= 2.0 ** -8 * (1 + 2.0 ** -8) * want.abs()).all()
