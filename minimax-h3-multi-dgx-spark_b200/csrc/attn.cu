@@ -430,8 +430,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     uint64_t *kv_full = bars, *kv_empty = bars + 4,  // of the groups
         *s_full = bars + 8, *p_full = bars + 12,     // [tile][buffer]
         *q_full = bars + 16, *q_empty = bars + 18, *pv_done = bars + 20, *o_full = bars + 22, *out_full = bars + 24,  // [tile]
-        *drain = bars + 26, *out_free = bars + 28, *take = bars + 29;  // [tile][scheduler]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 37);
+        *drain = bars + 26,
+        *out_free = bars + 28,  // the output's place: tile 0 to tile 1, tile 1 to tile 0, tile 0 to itself
+        *take = bars + 31;      // [tile][scheduler]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 39);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -455,7 +457,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             mbar_init(out_full + t, 4);
             mbar_init(drain + t, 1);
         }
-        mbar_init(out_free, 1);
+        for (int j = 0; j < 3; ++j) mbar_init(out_free + j, 1);
         for (int j = 0; j < 8; ++j) mbar_init(take + j, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -626,8 +628,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         const uint32_t at = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t tS = tmem + at + 128 * t, tO = tmem + at + 256 + 128 * t;
         const float scale2 = fabsf(a.scale) * kLog2e;
-        // this tile's steps and outputs so far, the uses of the output's place by both tiles, the steps of both
-        uint32_t step = 0, outs = 0, turn = 0, shared = 0;
+        // this tile's steps and outputs so far, the steps of both
+        uint32_t step = 0, outs = 0, shared = 0;
+        // items so far with both tiles and with tile 0 alone, which of the two the one before is
+        uint32_t pairs = 0, alone = 0;
+        bool after_pair = true;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t phase) {
             return __all_sync(0xFFFFFFFFu, await(bar, phase, abort_flag, a.status)) != 0;
@@ -636,10 +641,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             const Item it = item_of<SRC>(a, item);
             const Where u = where<SRC>(a, it.pair, t);
             const int32_t* list = list_of<SRC>(a, u);
-            // (uses of the place alternate: by the time of a tile's next one its former one is over, since all its warps
-            // have taken part in a step after it)
-            const uint32_t mine = turn + t;
-            turn += it.both ? 2 : 1;
+            // Each output waits for the one before it on the barrier of that hand-over: an item's second for its first, an
+            // item's first for the last of the item before (the CTA's very first passes at once).  One barrier for all of
+            // them would not do: a wait sees a phase's parity alone, and tile 1, which skips the items without it, could
+            // be two phases off.  A hand-over's next phase needs an output of its waiter in between, so it cannot be here.
+            uint64_t* const free_bar = out_free + (t == 1 ? 0 : after_pair ? 1 : 2);
+            const uint32_t free_phase = t == 1 ? pairs : (after_pair ? pairs : alone) - 1u;
+            if (it.both) ++pairs;
+            else ++alone;
+            after_pair = it.both;
             if (t == 1 && !it.both) continue;
             Row st{-INFINITY, 0.0f};
             struct Factors {
@@ -690,7 +700,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             const int64_t slot = ((int64_t)it.part * a.heads + u.h) * a.Sq + row;
             if (split && row < a.Sq) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(st.m, st.l);
             // the output's place is free when the store before has read it
-            if (!split && mine > 0 && !(ok = wait(out_free, mine - 1))) break;
+            if (!split && !(ok = wait(free_bar, free_phase))) break;
             // O: as it is to the join if this is a part of the keys, else through shared memory into whole rows of o
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
@@ -728,7 +738,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                         tma_store(&tmO, smem + L::kO, u.qt * kQRows, a.h0 + u.h);
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                         asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                        mbar_arrive(out_free);
+                        mbar_arrive(out_free + (t == 1 ? 1 : it.both ? 0 : 2));
                     }
                     __syncwarp();
                 }

@@ -615,3 +615,34 @@ def test_cached_attention_to_a_single_token_rounds_once(D, rows):
     got = h3b.kv8_attention(randn(rows, 5, D, seed=62), c).double()
     want = values(c)[1].expand(rows, -1, -1)
     assert ((got - want).abs() <= 2.0 ** -8 * (1 + 2.0 ** -8) * want.abs()).all()
+
+
+def items_of_a_head(rows):
+    """Pairs of row tiles of a head; the last has one tile only if the tiles are odd."""
+    return -(-rows // 256)
+
+
+def takes_a_single_tile_before_a_pair(rows, tokens, H, D):
+    """A CTA goes from an item with one tile to an item with both, and writes both to o itself (nothing is split)."""
+    each, sms = items_of_a_head(rows), torch.cuda.get_device_properties(DEV).multi_processor_count
+    whole = h3b.lib.h3b_attn_workspace(1, rows, H, D, -(-tokens // 64)) == 4 * H * -(-tokens // 64) * 64 * D
+    single = [i % each == each - 1 for i in range(each * H)]
+    return whole and -(-rows // 128) % 2 == 1 and any(a and not b for a, b in zip(single, single[sms:]))
+
+
+@pytest.mark.parametrize("tokens", [64, 77, 100, 128, 192, 256, 320])
+@pytest.mark.parametrize("rows,H,D", [(16000, 40, 128), (4128, 40, 128), (8000, 40, 128), (600, 100, 128), (600, 100, 64)])
+def test_cached_attention_outputs_after_an_item_with_a_single_tile(rows, tokens, H, D):
+    """Heads with an odd number of row tiles over short caches: both tiles of a CTA write their outputs through one
+    place, and after an item with tile 0 alone tile 1 is free to run ahead of it."""
+    assert takes_a_single_tile_before_a_pair(rows, tokens, H, D)
+    c = filled(H, -(-tokens // 64) * 64, D, tokens, seed=rows + tokens)
+    q = torch.randn(rows, H, D, generator=torch.Generator(device=DEV).manual_seed(tokens), device=DEV).bfloat16()
+    got = h3b.kv8_attention(q, c)
+    k, v = values(c)
+    for h in range(H):
+        o, a, m = softmax_rows(q[:, h], k[:, h], v[:, h], D ** -0.5)
+        near(got[:, h], o, a, m, tokens, D)
+    for _ in range(10):
+        assert torch.equal(h3b.kv8_attention(q, c), got)
+    assert h3b.status() == 0
