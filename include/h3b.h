@@ -255,9 +255,10 @@ H3B_API int h3b_gate_(void *x, const void *o, const void *g, const int32_t *ridx
  * codes kq, vq int8 [H, cap, D], scales ks, vs fp32 [H, cap / 64], cap % 64 == 0.
  * Per block of 64 tokens and head, K and V apart: s = max|x| / 127 over the new
  * tokens (IEEE division), or the block's former scale if tokens before `start`
- * stay in the block and it is larger; code = clamp(rint_half_even(x / s),
- * -127, 127), 0 for s = 0; staying codes become rint(code * (former / s)) if the
- * scale grew.  A NaN or infinity makes its block's scale non-finite and the
+ * stay in the block and it is larger in magnitude (a negative one stays
+ * negative); code = clamp(rint_half_even(x / s), -127, 127), 0 for s = 0;
+ * staying codes become rint(code * (former / s)) if the scale is not the former
+ * one.  A NaN or infinity makes its block's scale non-finite and the
  * codes 0.  Nothing behind start + n is written.  The cross-attention's K / V
  * projection is the same in every denoising step; the reference recomputes
  * it (the attention call of sp_forward.py:276-318). */

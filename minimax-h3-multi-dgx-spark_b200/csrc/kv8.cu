@@ -6,7 +6,9 @@
 // a scale) is 64 * D consecutive bytes.
 //
 //   scale = max |x| / 127 over the block's new tokens (IEEE division), or the
-//           block's older scale where older tokens stay and it is larger;
+//           block's older scale where older tokens stay and it is larger in
+//           magnitude (a cache that was not written here may have negative
+//           ones: the sign stays, as do the codes that go with it);
 //   code  = clamp(rint_half_even(x / scale), -127, 127), 0 for scale 0;
 //   codes that stay are requantised, rint(code * (old / scale)), if the scale grew.
 // A non-finite x makes the scale non-finite and the block's codes 0, so
@@ -79,7 +81,7 @@ __global__ void __launch_bounds__(kWriteThreads) write_kernel(const __grid_const
     // a NaN's quotient is a NaN: the order of the bit patterns still holds below
     float s = __fdiv_rn(__uint_as_float(top), 127.0f);
     if ((__float_as_uint(older) & 0x7FFFFFFFu) > (__float_as_uint(s) & 0x7FFFFFFFu)) s = older;
-    const bool live = s > 0.0f && s < __int_as_float(0x7F800000);
+    const bool live = s != 0.0f && fabsf(s) < __int_as_float(0x7F800000);
     const float inverse = live ? __frcp_rn(s) : 0.0f;
     const bool grew = stays && __float_as_uint(s) != __float_as_uint(older);
     const float ratio = grew && live ? __fdiv_rn(older, s) : 0.0f;
@@ -90,7 +92,7 @@ __global__ void __launch_bounds__(kWriteThreads) write_kernel(const __grid_const
         if (r >= first && r < last) {
             float f[8];
             unpack8(v[p], f);
-            // (the scale is the block's absmax / 127 or larger, so no code leaves [-127, 127])
+            // (the scale's magnitude is the block's absmax / 127 or larger, so no code leaves [-127, 127])
             *dst = live ? quant8(f, s, inverse) : make_uint2(0u, 0u);
         } else if (grew && r < first) {
             const uint2 old = *dst;

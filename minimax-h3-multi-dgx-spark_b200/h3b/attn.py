@@ -139,8 +139,8 @@ class KV8Cache:
     def write(self, k, v, start=None):
         """Quantise k, v [n, heads, head_dim] (bf16) into tokens start .. start + n (start <= length, by default the
         end); tokens that lay at and behind start are dropped.  A block's scale is its new tokens' absmax / 127, or
-        its former scale where older tokens stay in it and that is larger; staying codes are requantised when the
-        scale grows.  A NaN or infinity makes its block and head NaN.  Returns the cache."""
+        its former scale where older tokens stay in it and that is larger in magnitude; staying codes are requantised
+        when the scale changes.  A NaN or infinity makes its block and head NaN.  Returns the cache."""
         require_cuda(k, v)
         start = self.length if start is None else int(start)
         (kld, khs), (vld, vhs) = _rows("k", k), _rows("v", v, k)

@@ -646,3 +646,49 @@ def test_cached_attention_outputs_after_an_item_with_a_single_tile(rows, tokens,
     for _ in range(10):
         assert torch.equal(h3b.kv8_attention(q, c), got)
     assert h3b.status() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("start,n", [(17, 1), (100, 28), (63, 200)])
+def test_write_behind_scales_of_either_sign(D, start, n):
+    """The staying tokens' scale is kept if it is larger in magnitude, of whichever sign, and gives way if it is not."""
+    H, block = 8, start // 64
+    c = filled(H, -(-(start + n) // 64) * 64, D, start, seed=71)
+    k, v = randn(n, H, D, seed=72), randn(n, H, D, seed=73)
+    factor = torch.tensor([0.5, -0.5, 2.0, -2.0, -1.0, -0.01, 30.0, -30.0])
+    before, want = [], []
+    for x, codes, scales in ((k, c.kq, c.ks), (v, c.vq, c.vs)):
+        here = x[:64 - start % 64].float().cpu().transpose(0, 1)  # the new tokens of the block that holds older ones
+        new = here.abs().amax((1, 2)) / torch.tensor(127.0)
+        former = new * factor
+        scales[:, block] = former.to(DEV)
+        old = codes[:, block * 64:start].float().cpu()
+        s = torch.where(former.abs() > new, former, new)
+        kept = torch.where((s == former)[:, None, None], old, (old * (former / s)[:, None, None]).round())
+        before.append(old.double() * former.double()[:, None, None])
+        want.append((torch.cat([kept, (here / s[:, None, None]).round()], 1), s))
+    c.write(k, v)
+    end = min(start + n, block * 64 + 64)
+    for codes, scales, (q, s), was, x in zip((c.kq, c.vq), (c.ks, c.vs), want, before, (k, v)):
+        assert same(codes[:, block * 64:end].float(), q) and same(scales[:, block], s)
+        # what is held is off by half a step of the code and three fp32 roundings at 127 steps
+        step = s.double().abs()[:, None, None] * (0.5 + 3 * 127 * 2.0 ** -24)
+        got = codes[:, block * 64:end].double().cpu() * s.double()[:, None, None]
+        now = torch.cat([was, x[:end - start].double().cpu().transpose(0, 1)], 1)
+        assert ((got - now).abs() <= step).all()
+    check_cached(randn(3, H, D, seed=74), c)
+    check_cached(randn(70, H, D, seed=75), c)
+
+
+@pytest.mark.parametrize("former", [-0.0, -INF, NAN])
+def test_write_behind_scales_that_are_no_numbers(former):
+    c = filled(2, 64, 64, 10, seed=76)
+    c.ks[0], c.vs[0] = former, former
+    x = randn(5, 2, 64, seed=77)
+    gk, gv = c.write(x, x).read(dtype=torch.float32)
+    for g in (gk, gv):
+        if former == 0:
+            assert (g[:10, 0] == 0).all() and (g[10:, 0] != 0).any()
+        else:
+            assert torch.isnan(g[10:, 0]).all() and not torch.isfinite(g[:10, 0]).any()
+        assert torch.isfinite(g[:, 1]).all()
