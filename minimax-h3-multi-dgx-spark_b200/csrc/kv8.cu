@@ -184,8 +184,9 @@ extern "C" int h3b_kv8_write(const void* k, int64_t k_ld, int64_t k_hs, const vo
     if (int rc = kv8::check_cache("h3b_kv8_write", kq, vq, ks, vs, cap, start, n, H, D)) return rc;
     if (n == 0) return H3B_OK;
     H3B_REQUIRE(k && v && aligned(k, 16) && aligned(v, 16), "h3b_kv8_write: k / v NULL or not 16-byte aligned");
-    H3B_REQUIRE(k_ld % 8 == 0 && k_hs % 8 == 0 && v_ld % 8 == 0 && v_hs % 8 == 0,
-                "h3b_kv8_write: token and head strides must be multiples of 8 elements");
+    H3B_REQUIRE(k_ld > 0 && k_hs > 0 && v_ld > 0 && v_hs > 0 && k_ld % 8 == 0 && k_hs % 8 == 0 && v_ld % 8 == 0 &&
+                    v_hs % 8 == 0,
+                "h3b_kv8_write: token and head strides must be positive multiples of 8 elements");
     kv8::WriteArgs a{{static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v)},
                      {k_ld, v_ld}, {k_hs, v_hs}, {kq, vq}, {ks, vs}, cap, start, n, (int)H};
     const int64_t blocks = cdiv(start + n, kv8::kBlock) - start / kv8::kBlock;

@@ -117,8 +117,8 @@ static int check_means(const char* who, const void* x, int64_t ld, int64_t hs, i
                        float* out, Means* m) {
     *m = Means{static_cast<const uint16_t*>(x), ld, hs, S, out, cdiv(S, rows) * H};
     if (S == 0) return H3B_OK;
-    H3B_REQUIRE(x && out && aligned(x, 16) && ld % 8 == 0 && hs % 8 == 0,
-                "%s: x / out NULL, x not 16-byte aligned or strides not multiples of 8 elements", who);
+    H3B_REQUIRE(x && out && aligned(x, 16) && ld > 0 && hs > 0 && ld % 8 == 0 && hs % 8 == 0,
+                "%s: x / out NULL, x not 16-byte aligned or strides not positive multiples of 8 elements", who);
     H3B_REQUIRE(m->ctas < (1ll << 30), "%s: too many blocks", who);
     return H3B_OK;
 }

@@ -140,3 +140,15 @@ def test_python_checks_on_the_cpu():
             h3b.KV8Cache.wrap(*bad)
     with pytest.raises(TypeError):
         h3b.KV8Cache.wrap(kq, kq, ks, ks, 0)
+
+
+def test_strides_must_be_positive():
+    for stride in (0, -128):
+        refused("h3b_kv8_write", write(kld=stride), "strides")
+        refused("h3b_kv8_write", write(khs=stride), "strides")
+        refused("h3b_kv8_write", lib.h3b_kv8_write(P16, 128, 128, P16, stride, 128, 0, 1, 1, 128, P16, P16, P16, P16, 64, P0),
+                "strides")
+        refused("h3b_kv8_write", lib.h3b_kv8_write(P16, 128, 128, P16, 128, stride, 0, 1, 1, 128, P16, P16, P16, P16, 64, P0),
+                "strides")
+        refused("h3b_block_means", lib.h3b_block_means(P16, stride, 128, 5, 1, 128, 64, P16, P0), "strides")
+        refused("h3b_block_means", lib.h3b_block_means(P16, 128, stride, 5, 1, 128, 64, P16, P0), "strides")
