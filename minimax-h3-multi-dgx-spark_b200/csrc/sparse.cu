@@ -56,6 +56,12 @@ extern "C" int h3b_sparse_attn(const void* q, int64_t q_ld, int64_t q_hs, int64_
     H3B_REQUIRE(l.bytes == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= l.bytes),
                 "h3b_sparse_attn: workspace of %lld bytes (256-byte aligned), %lld needed", (long long)workspace_bytes,
                 (long long)l.bytes);
+    // (what the attention would refuse, before the means and the selection are under way)
+    H3B_REQUIRE(Sq == 0 || (q && o && aligned(q, 16) && aligned(o, 16)), "h3b_sparse_attn: q / o NULL or not 16-byte aligned");
+    H3B_REQUIRE(Sk == 0 || (k && v && aligned(k, 16) && aligned(v, 16)), "h3b_sparse_attn: k / v NULL or not 16-byte aligned");
+    H3B_REQUIRE(Sq == 0 || l.topk == 0 || (blocks && aligned(blocks, 4)), "h3b_sparse_attn: blocks NULL");
+    for (const int64_t stride : {q_ld, q_hs, k_ld, k_hs, v_ld, v_hs, o_ld, o_hs})
+        H3B_REQUIRE(stride > 0 && stride % 8 == 0, "h3b_sparse_attn: strides must be positive multiples of 8 elements");
     char* ws = static_cast<char*>(workspace);
     float *qm = reinterpret_cast<float*>(ws + l.qm), *km = reinterpret_cast<float*>(ws + l.km);
     if (l.topk > 0 && Sq > 0) {

@@ -152,3 +152,18 @@ def test_strides_must_be_positive():
                 "strides")
         refused("h3b_block_means", lib.h3b_block_means(P16, stride, 128, 5, 1, 128, 64, P16, P0), "strides")
         refused("h3b_block_means", lib.h3b_block_means(P16, 128, stride, 5, 1, 128, 64, P16, P0), "strides")
+
+
+def test_sparse_attention_is_refused_before_any_of_its_steps():
+    """The attention's own checks come before the means and the selection are enqueued (no device here to run them)."""
+    def sparse(q=P16, k=P16, v=P16, o=P16, blocks=P16, **stride):
+        st = {**dict.fromkeys(("qld", "kld", "vld", "old"), 256), **dict.fromkeys(("qhs", "khs", "vhs", "ohs"), 128), **stride}
+        return lib.h3b_sparse_attn(q, st["qld"], st["qhs"], 200, 2, 128, k, st["kld"], st["khs"], v, st["vld"], st["vhs"], 100,
+                                   P0, 2, 1.0, blocks, o, st["old"], st["ohs"], P16, 1 << 30, P0)
+    for bad in (P0, P2):
+        for name in "qkvo":
+            refused("h3b_sparse_attn", sparse(**{name: bad}), "aligned")
+    refused("h3b_sparse_attn", sparse(blocks=P0), "blocks")
+    for name in ("qld", "qhs", "kld", "khs", "vld", "vhs", "old", "ohs"):
+        for stride in (0, -256, 132):
+            refused("h3b_sparse_attn", sparse(**{name: stride}), "strides")
