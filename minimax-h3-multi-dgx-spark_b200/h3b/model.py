@@ -279,8 +279,9 @@ class SynthDiT:
 
     def forward(self, x, ridx, ctx=None, text=None):
         """text: the text tokens [t, D], the list that text_cache gives, or None."""
-        if isinstance(text, (list, tuple)) and len(text) != len(self.params):
-            raise ValueError(f"SynthDiT.forward: {len(text)} text caches for {len(self.params)} blocks")
+        n = len(text) if isinstance(text, (list, tuple)) else 1 if isinstance(text, attn.KV8Cache) else None
+        if n is not None and n != len(self.params):  # (a cache holds the keys and values of one block)
+            raise ValueError(f"SynthDiT.forward: {n} text caches for {len(self.params)} blocks")
         for i, p in enumerate(self.params):
             x = block_forward(self.cfg, p, x, ridx, ctx, text[i] if isinstance(text, (list, tuple)) else text)
         return x

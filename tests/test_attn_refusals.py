@@ -167,3 +167,15 @@ def test_sparse_attention_is_refused_before_any_of_its_steps():
     for name in ("qld", "qhs", "kld", "khs", "vld", "vhs", "old", "ohs"):
         for stride in (0, -256, 132):
             refused("h3b_sparse_attn", sparse(**{name: stride}), "strides")
+
+
+def test_a_single_text_cache_is_not_taken_for_several_blocks():
+    """A cache holds one block's keys and values: given alone it would serve every block with those."""
+    from h3b import model as hm
+
+    dit = object.__new__(hm.SynthDiT)
+    dit.cfg, dit.params = None, [None, None]
+    cache = object.__new__(h3b.KV8Cache)
+    for text in (cache, [cache], (cache,) * 3):
+        with pytest.raises(ValueError, match="text caches for 2 blocks"):
+            dit.forward(None, None, None, text)
