@@ -311,7 +311,7 @@ H3B_API int h3b_select_blocks(const float *qm, const float *km, int64_t nq, int6
  * the keys of blocks[h, i, 0 .. topk) only; block b holds keys 64 b .. 64 b + 63
  * below Sk.  -1 is no block; another index out of range is skipped and recorded
  * as H3B_STATUS_BAD_INDEX; a block named twice counts twice; rows without a key
- * are zero.  Replaces the scaled_dot_product_attention of sp_forward.py:276-318. */
+ * are zero (rows whose scores are all -infinity NaN, as in h3b_kv8_attn).  Replaces the scaled_dot_product_attention of sp_forward.py:276-318. */
 H3B_API int h3b_block_sparse_attn(const void *q, int64_t q_ld, int64_t q_hs, int64_t Sq, int64_t H, int64_t D,
                                   const void *k, int64_t k_ld, int64_t k_hs, const void *v, int64_t v_ld,
                                   int64_t v_hs, int64_t Sk, const int32_t *blocks, int64_t topk, float scale,

@@ -64,6 +64,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // stays below 2^8, far from any limit of fp32 or bf16 (whose relative
 // precision does not depend on it), and O is not rescaled.
 constexpr float kSlack = 8.0f;
+// The maximum that a part of a split passes on where it has keys whose scores are all
+// -infinity; -infinity itself: no keys.  (Rows without a key are zero, rows of such scores NaN.)
+constexpr float kLowest = -3.402823466e38f;
 
 template <int D>
 struct Smem {
@@ -664,9 +667,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 return Factors{g.n, fabsf(__ldg(a.scales[0] + b)), a.segs == 1 ? 1.0f : __ldg(a.scales[1] + b)};
             };
             Factors ahead = factors(0);
+            bool keys = SRC == kWide;  // the part has some
             const bool paired = it.both && a.turns;
             for (int i = 0; ok && i < it.steps; ++i, ++step) {
                 const Factors f = ahead;
+                if (SRC == kBlocks) keys |= f.n > 0;
                 // tile 1 follows tile 0's exponentials of the same step, tile 0 tile 1's of the step before
                 const Turn turns{paired ? take + (warp & 3) + 4 * t : nullptr, take + (warp & 3) + 4 * (1 - t),
                                  shared + t - 1u, abort_flag, a.status};
@@ -693,12 +698,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             tc_fence_after();
             const int64_t row = (int64_t)u.qt * kQRows + trow;
             const bool split = a.parts > 1;
-            float inv = st.l == 0.0f ? 0.0f : 1.0f / st.l;
+            float inv = keys ? 1.0f / st.l : 0.0f;
             // (one block: its scale is not rounded with p, whose rounding would be that of every output of a head where
             // there is one token)
             if (SRC == kWide && a.segs == 1) inv *= __ldg(a.scales[1] + (int64_t)(a.h0 + u.h) * (a.cap / kSeg));
             const int64_t slot = ((int64_t)it.part * a.heads + u.h) * a.Sq + row;
-            if (split && row < a.Sq) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(st.m, st.l);
+            if (split && row < a.Sq)
+                *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(keys ? fmaxf(st.m, kLowest) : st.m, st.l);
             // the output's place is free when the store before has read it
             if (!split && !(ok = wait(free_bar, free_phase))) break;
             // O: as it is to the join if this is a part of the keys, else through shared memory into whole rows of o
@@ -1044,9 +1050,9 @@ __global__ void __launch_bounds__(32 * WARPS, row_ctas(D, GROUPS) * kRowWarps / 
         if (a.parts > 1) {
             const int64_t slot = ((int64_t)part * a.H + h) * a.Sq + row0 + r;
             *reinterpret_cast<float2*>(a.part_o + slot * D + ch) = make_float2(x, y);
-            if (ch == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(top, total);
+            if (ch == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * slot) = make_float2(fmaxf(top, kLowest), total);
         } else {
-            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            const float inv = 1.0f / total;
             *reinterpret_cast<uint32_t*>(a.o + (row0 + r) * a.o_ld + h * a.o_hs + ch) = pack_bf16x2(x * inv, y * inv);
         }
     }
@@ -1083,7 +1089,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args 
     if (threadIdx.x < D / 2) {
         const int ch = 2 * threadIdx.x;
         const float total = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        const float inv = m == -INFINITY ? 0.0f : 1.0f / total;
         float x[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) x[e] = ((so[0][ch + e] + so[1][ch + e]) + (so[2][ch + e] + so[3][ch + e])) * inv;

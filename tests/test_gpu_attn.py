@@ -692,3 +692,40 @@ def test_write_behind_scales_that_are_no_numbers(former):
         else:
             assert torch.isnan(g[10:, 0]).all() and not torch.isfinite(g[:10, 0]).any()
         assert torch.isfinite(g[:, 1]).all()
+
+
+@pytest.mark.parametrize("rows", [1, 20, 70, 300])
+@pytest.mark.parametrize("tokens", [1, 64, 3000])
+def test_cached_attention_of_rows_whose_scores_are_all_minus_infinity(rows, tokens):
+    """A softmax over nothing but -infinity is NaN, whole and split over the keys; a row that has keys is never zeros."""
+    c = filled(2, -(-tokens // 64) * 64, 128, tokens, seed=81)
+    c.kq[:, :tokens, 0] = -5
+    q = randn(rows, 2, 128, seed=82)
+    want = h3b.kv8_attention(q, c)
+    q[rows // 2, 1, 0] = INF
+    got = h3b.kv8_attention(q, c)
+    assert torch.isnan(got[rows // 2, 1]).all()
+    got[rows // 2, 1] = want[rows // 2, 1]
+    assert same(got, want)
+
+
+@pytest.mark.parametrize("rows,topk", [(1, 3), (1, 130), (300, 3), (300, 40)])
+def test_sparse_attention_over_scores_of_minus_infinity(rows, topk):
+    """Keys with a score of -infinity weigh nothing beside others; rows that have no other are NaN, rows that have no key
+    at all zero."""
+    H, D, keys, nq = 2, 128, 9000, -(-rows // 128)
+    q, k, v = randn(rows, H, D, seed=83), randn(keys, H, D, seed=84), randn(keys, H, D, seed=85)
+    q[:, :, 0] = 1.0
+    k[64:, 1, 0] = -INF  # all blocks of head 1 but the first
+    blocks = torch.arange(topk, dtype=torch.int32, device=DEV).expand(H, nq, topk).contiguous()
+    got = h3b.block_sparse_attention(q, k, v, blocks)
+    alone = torch.full_like(blocks, -1)
+    alone[0], alone[1, :, 0] = blocks[0], 0
+    o, a, m = sparse(q, k, v, alone, D ** -0.5)
+    near(got, o, a, m, topk * 64, D)
+    blocks[1, :, 0] = -1
+    got = h3b.block_sparse_attention(q, k, v, blocks)
+    assert torch.isnan(got[:, 1]).all() and torch.isfinite(got[:, 0]).all()
+    blocks[1] = -1
+    assert (h3b.block_sparse_attention(q, k, v, blocks)[:, 1] == 0).all()
+    assert h3b.status() == 0
