@@ -292,7 +292,8 @@ H3B_API int h3b_kv8_attn(const void *q, int64_t q_ld, int64_t q_hs, int64_t Sq, 
 
 /* out[b, h, :] = mean of rows b * rows .. of x [S, H, D] bf16 (rows 64 or 128;
  * the last block over the rows it has) -> fp32 [ceil(S / rows), H, D], summed
- * in 64 bits and rounded once.  The cheap score of block-sparse attention in
+ * in 64 bits and rounded once (exact while a block's nonzero values lie within a
+ * factor of 2^38).  The cheap score of block-sparse attention in
  * place of the dense one of sp_forward.py:276-318. */
 H3B_API int h3b_block_means(const void *x, int64_t ld, int64_t hs, int64_t S, int64_t H, int64_t D, int64_t rows,
                             float *out, void *stream);

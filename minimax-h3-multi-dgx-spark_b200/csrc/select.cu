@@ -1,11 +1,15 @@
 // Selection of key blocks for block-sparse attention: the means of blocks of
 // rows, the products of the means, and the top-k of each (head, query block).
 //
-// A selection hangs on differences between scores, so nothing here may depend
-// on the order of a sum: means are summed in 64 bits (bf16 values of one block
-// add up exactly there) and rounded once to 32 bits; scores are sums of exact
-// products in 64 bits; equal scores go to the lowest index.  A NaN score ranks
-// below every number, -0 equals +0.
+// A selection hangs on differences between scores, so sums are held in 64 bits:
+// means are rounded once to 32 bits; scores are sums of exact products; equal
+// scores go to the lowest index.  A NaN score ranks below every number, -0
+// equals +0.  Where a sum fits 53 bits its order does not matter: a block of 128
+// rows whose nonzero values lie within a factor of 2^38 (8 + 38 bits and 7 for
+// the carries) has the same mean in any order.  Beyond, and in the scores, an
+// order may change the last bits of the 64; each kernel's own is fixed, but
+// score_kernel and score_few_kernel have different ones, and so may rank blocks
+// differently whose scores are equal but for that.
 #include "quant_common.cuh"
 
 namespace h3b {

@@ -196,8 +196,8 @@ def kv8_attention(q, cache, scale=None):
 
 def block_means(x, rows=KEYS, out=None):
     """fp32 [ceil(n / rows), heads, head_dim]: the mean of each block of `rows` (64 or 128) rows of x
-    [n, heads, head_dim] bf16, the last block's over the rows it has.  Summed in 64 bits and rounded once, so it does
-    not depend on an order.  out (optional, contiguous) takes the result: a program that appends keys keeps the means
+    [n, heads, head_dim] bf16, the last block's over the rows it has.  Summed in 64 bits and rounded once: exact sums
+    where a block's nonzero values lie within a factor of 2^38, a fixed order otherwise.  out (optional, contiguous) takes the result: a program that appends keys keeps the means
     and renews those of the blocks it touched, block_means(k[64 * b:], out=means[b:])."""
     require_cuda(x)
     ld, hs = _rows("x", x)
@@ -218,7 +218,8 @@ def block_means(x, rows=KEYS, out=None):
 def select_blocks(qm, km, topk):
     """int32 [heads, nq, min(topk, nk)]: for each head and row of qm [nq, heads, head_dim] (fp32 means of query
     blocks) the rows of km [nk, heads, head_dim] with the largest products, ascending.  Products are summed in 64
-    bits; ties go to the lowest index, a NaN product ranks below every number."""
+    bits (in an order of their own up to 4 query blocks: scores that differ by no more than its rounding may rank
+    either way); ties go to the lowest index, a NaN product ranks below every number."""
     require_cuda(qm, km)
     if qm.dim() != 3 or km.dim() != 3 or qm.shape[1:] != km.shape[1:] or qm.device != km.device:
         raise ValueError(f"select_blocks: means {tuple(qm.shape)} and {tuple(km.shape)} do not go together")

@@ -729,3 +729,15 @@ def test_sparse_attention_over_scores_of_minus_infinity(rows, topk):
     blocks[1] = -1
     assert (h3b.block_sparse_attention(q, k, v, blocks)[:, 1] == 0).all()
     assert h3b.status() == 0
+
+
+@pytest.mark.parametrize("rows", [64, 128])
+def test_block_means_of_any_order_within_their_exact_range(rows):
+    """Values within a factor of 2^38 add up to 53 bits at most (8 + 38 + 7), so a block's mean is that of its rows in any
+    order."""
+    x = randn(rows, 3, 128, seed=91).float().sign() * (1 + torch.rand(rows, 3, 128, generator=gen(92))).to(DEV)
+    x = (x * 2.0 ** torch.randint(-19, 19, (rows, 3, 128), generator=gen(93)).to(DEV)).bfloat16()
+    want = h3b.block_means(x, rows)
+    assert same(want, means(x, rows))
+    for seed in range(5):
+        assert torch.equal(h3b.block_means(x[torch.randperm(rows, generator=gen(94 + seed)).to(DEV)], rows), want)
