@@ -53,9 +53,11 @@ struct Args {
 // tensor cores wait for a chain to go round.  (One S of 128 columns a tile, the
 // other form that fits in TMEM, left the tensor cores idle more than half of the
 // time: the chain of a step took 3700 clocks, of which 1024 are products.)
-// Bound by shared memory: the operands of Q K^T alone take its 128 bytes a clock
-// for 384 clocks a step and tile, where the products take 256.  128000 rows of 5
-// heads over 64 blocks each: 1.28 ms, 1050 TFLOP/s.
+// What bounds it: shared memory in part (the operands of Q K^T alone take its 128
+// bytes a clock for 384 clocks a step and tile, where the products take 256: 1280
+// clocks a step of both tiles), the chain of a step and the power cap for the
+// rest (1950 measured).  128000 rows of 5 heads over 64 blocks each: 1.28 ms, 1050
+// TFLOP/s.
 
 constexpr int kTmemCols = 512;     // S of tile t at 128 t (+ 64 for odd steps), O at 256 + 128 t
 constexpr int kPairThreads = 384;  // 2 x 4 softmax warps, an MMA warp and a TMA warp for each tile
@@ -283,7 +285,6 @@ struct Turn {
         if (mine && (threadIdx.x & 31) == 0) mbar_arrive(other);
     }
 };
-constexpr int kPassOn = 1;  // half of a step's exponentials before which the turn passes on (2: behind them)
 
 // One step of a row: S (64 columns at tS) -> P (bf16, 32 columns at tS), with the
 // running maximum and sum.  n: valid keys; sk, sv: factors of the scores (softmax
@@ -337,7 +338,7 @@ __device__ __forceinline__ void softmax_step(Row& st, uint32_t tS, uint32_t tO, 
     turn.take(seen);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-        if (c == kPassOn) turn.pass();
+        if (c == 1) turn.pass();  // (before the second half of the exponentials)
         uint32_t p[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -356,7 +357,6 @@ __device__ __forceinline__ void softmax_step(Row& st, uint32_t tS, uint32_t tO, 
         }
         tmem_st16(tS + c * 16, p);
     }
-    if (kPassOn == 2) turn.pass();
     sum[0] = add2(sum[0], sum[1]);
     st.l += sum[0].x + sum[0].y;
 }
