@@ -741,3 +741,21 @@ def test_block_means_of_any_order_within_their_exact_range(rows):
     assert same(want, means(x, rows))
     for seed in range(5):
         assert torch.equal(h3b.block_means(x[torch.randperm(rows, generator=gen(94 + seed)).to(DEV)], rows), want)
+
+
+@pytest.mark.parametrize("rows,H,groups,topk", [(700, 4, 2, 3), (20000, 40, 8, 4)])
+def test_sparse_attention_of_head_groups_selects_the_same_blocks(rows, H, groups, topk):
+    """Calls of some heads each, on views of one buffer as a head group's exchange delivers them: the blocks are those of
+    the call of all heads; the outputs are right, if not bitwise the same (a call's split over the keys goes by its heads)."""
+    hc, D = H // groups, 64
+    buf = [randn(rows * H * D, seed=s) for s in (101, 102, 103)]
+    views = [[b[g * rows * hc * D:(g + 1) * rows * hc * D].view(rows, hc, D) for b in buf] for g in range(groups)]
+    q, k, v = (torch.cat([views[g][i] for g in range(groups)], 1) for i in range(3))
+    o, blocks = h3b.sparse_attention(q, k, v, topk, return_blocks=True)
+    for g in (0, groups - 1):
+        og, bg = h3b.sparse_attention(*views[g], topk, return_blocks=True)
+        assert same(bg, blocks[g * hc:(g + 1) * hc])
+        ref, a, m = sparse(*(t[:, :1] for t in views[g]), bg[:1], D ** -0.5)
+        near(og[:, :1], ref, a, m, topk * 64, D)
+        near(o[:, g * hc:g * hc + 1], ref, a, m, topk * 64, D)
+    assert h3b.status() == 0
